@@ -6,6 +6,10 @@ Drop-in surface (same names as the reference):
     from afa_py.afa_config import AFAForwardKernelConfig
     O, ms = fa.forward(AFAForwardKernelConfig(), q, k, v, o, benchmark)
 
+Beside it: ``forward_ext`` (causal mask, grouped heads), ``forward_host``, and for serving
+and training around it ``rotary``, ``cache4_write``, ``cache4_read`` and ``forward_cache4``
+(rotary positions, a paged 4-bit key/value cache and attention over it).
+
 ``forward`` runs the hand-written tcgen05/TMA kernel in ``libafa_sm100.so``;
 there is no other implementation behind it.  If the native extension is not
 built, importing ``forward`` raises ImportError (build with
@@ -35,6 +39,17 @@ def _load_extension():
 
 
 def __getattr__(name):
-    if name in ("forward", "forward_ext", "forward_host", "check_status", "kernel_keys"):
+    if name in (
+        "forward",
+        "forward_ext",
+        "forward_host",
+        "rotary",
+        "cache4_empty",
+        "cache4_write",
+        "cache4_read",
+        "forward_cache4",
+        "check_status",
+        "kernel_keys",
+    ):
         return getattr(_load_extension(), name)
     raise AttributeError(name)

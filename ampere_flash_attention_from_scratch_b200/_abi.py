@@ -32,6 +32,12 @@ AFA_NOALLOC_SCRATCH_BYTES = 256
 AFA_TEST_PRODUCER_IDLE = 1
 AFA_TEST_MMA_IDLE = 2
 AFA_TEST_KEEP_SCHED = 4
+AFA_DEV_BAD_PAGE = 0x201
+AFA_DEV_BAD_LENGTH = 0x202
+AFA_POS_INT32 = 0
+AFA_POS_INT64 = 1
+AFA_POS_FP32 = 2
+AFA_ROTARY_MAX_AXES = 8
 
 # Every extern "C" symbol declared in include/afa_sm100.h.
 EXPORTED_SYMBOLS = (
@@ -43,6 +49,17 @@ EXPORTED_SYMBOLS = (
     "afa_fwd_sm100_smem_bytes",
     "afa_fwd_sm100_threads",
     "afa_sm100_version",
+)
+
+# Every extern "C" symbol declared in include/afa_sm100_ops.h.
+EXPORTED_OPS_SYMBOLS = (
+    "afa_rotary_sm100",
+    "afa_cache4_write_sm100",
+    "afa_cache4_read_sm100",
+    "afa_cache4_fwd_workspace",
+    "afa_cache4_fwd_sm100",
+    "afa_cache4_row_bytes",
+    "afa_sm100_ops_version",
 )
 
 
@@ -73,6 +90,71 @@ class AfaFwdArgs(ctypes.Structure):
     ]
 
 
+class AfaRotaryArgs(ctypes.Structure):
+    """include/afa_sm100_ops.h, as are the two below."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("q_out_strides", ctypes.c_int64 * 3),
+        ("k_out_strides", ctypes.c_int64 * 3),
+        ("positions", ctypes.c_void_p),
+        ("pos_strides", ctypes.c_int64 * 3),
+        ("inv_freq", ctypes.c_void_p),
+        ("sections", ctypes.c_int32 * AFA_ROTARY_MAX_AXES),
+        ("n_axes", ctypes.c_int32),
+        ("pos_type", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("n_k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rot_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+    ]
+
+
+class AfaCache4(ctypes.Structure):
+    _fields_ = [
+        ("cache", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("kv_lens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class AfaCache4FwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("o_strides", ctypes.c_int64 * 3),
+        ("lse", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("seq_len", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 _lib = None
 
 
@@ -99,6 +181,21 @@ def load() -> ctypes.CDLL:
         lib.afa_fwd_sm100_threads.restype = ctypes.c_int
         lib.afa_sm100_version.argtypes = []
         lib.afa_sm100_version.restype = ctypes.c_int
+        strides = ctypes.POINTER(ctypes.c_int64)
+        lib.afa_rotary_sm100.argtypes = [ctypes.POINTER(AfaRotaryArgs), ctypes.c_void_p]
+        lib.afa_rotary_sm100.restype = ctypes.c_int
+        for move in (lib.afa_cache4_write_sm100, lib.afa_cache4_read_sm100):
+            move.argtypes = [ctypes.POINTER(AfaCache4), ctypes.c_void_p, ctypes.c_void_p, strides, strides, ctypes.c_int32,
+                             ctypes.c_void_p]
+            move.restype = ctypes.c_int
+        lib.afa_cache4_fwd_workspace.argtypes = [ctypes.POINTER(AfaCache4), ctypes.c_int32, ctypes.c_int32]
+        lib.afa_cache4_fwd_workspace.restype = ctypes.c_int64
+        lib.afa_cache4_fwd_sm100.argtypes = [ctypes.POINTER(AfaCache4), ctypes.POINTER(AfaCache4FwdArgs), ctypes.c_void_p]
+        lib.afa_cache4_fwd_sm100.restype = ctypes.c_int
+        lib.afa_cache4_row_bytes.argtypes = [ctypes.c_int32]
+        lib.afa_cache4_row_bytes.restype = ctypes.c_int32
+        lib.afa_sm100_ops_version.argtypes = []
+        lib.afa_sm100_ops_version.restype = ctypes.c_int
         _lib = lib
     return _lib
 

@@ -32,6 +32,10 @@ INCLUDE = REPO / "include"
 LIB_NAME = "libafa_sm100.so"
 EXT_NAME = "afa_flash_attention_kernels"
 
+# Translation units of the library and of the torch extension.
+LIB_UNITS = ("afa_fwd_sm100.cu", "afa_rotary_sm100.cu", "afa_cache4_sm100.cu", "afa_cache4_fwd_sm100.cu")
+EXT_UNITS = ("afa_torch_binding.cpp", "afa_torch_ops.cpp")
+
 NVCC_FLAGS = [
     "-gencode",
     "arch=compute_100a,code=sm_100a",
@@ -95,16 +99,19 @@ def extension_path() -> Path:
 def build_library(force: bool = False, verbose: bool = False) -> Path:
     inc = generate_presets()
     out = library_path()
+    units = [CSRC / name for name in LIB_UNITS]
     sources = [
-        CSRC / "afa_fwd_sm100.cu",
+        *units,
         CSRC / "afa_fwd_kernel.cuh",
+        CSRC / "ops_common.cuh",
         CSRC / "sm100_ptx.cuh",
         inc,
         INCLUDE / "afa_sm100.h",
+        INCLUDE / "afa_sm100_ops.h",
     ]
     if force or _stale(out, sources):
         tmp = out.with_suffix(".so.tmp")
-        cmd = [_nvcc(), *NVCC_FLAGS, "-shared", f"-I{INCLUDE}", f"-I{CSRC}", "-o", tmp, CSRC / "afa_fwd_sm100.cu"]
+        cmd = [_nvcc(), *NVCC_FLAGS, "--threads", "0", "-shared", f"-I{INCLUDE}", f"-I{CSRC}", "-o", tmp, *units]
         _run(cmd, verbose)
         os.replace(tmp, out)
     return out
@@ -116,7 +123,8 @@ def build_extension(force: bool = False, verbose: bool = False) -> Path:
 
     lib = build_library(force=force, verbose=verbose)
     out = extension_path()
-    sources = [CSRC / "afa_torch_binding.cpp", INCLUDE / "afa_sm100.h", lib]
+    units = [CSRC / name for name in EXT_UNITS]
+    sources = [*units, CSRC / "afa_torch_common.h", INCLUDE / "afa_sm100.h", INCLUDE / "afa_sm100_ops.h", lib]
     if not (force or _stale(out, sources)):
         return out
     cuda_home = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
@@ -134,7 +142,8 @@ def build_extension(force: bool = False, verbose: bool = False) -> Path:
         f"-DTORCH_EXTENSION_NAME={EXT_NAME}",
         "-DTORCH_API_INCLUDE_EXTENSION_H",
         *[f"-I{p}" for p in includes],
-        CSRC / "afa_torch_binding.cpp",
+        f"-I{CSRC}",
+        *units,
         "-o",
         out.with_suffix(".tmp"),
         f"-L{PKG}",

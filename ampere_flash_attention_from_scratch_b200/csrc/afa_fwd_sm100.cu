@@ -26,6 +26,7 @@
 
 #include "afa_fwd_kernel.cuh"
 #include "afa_sm100.h"
+#include "afa_sm100_ops.h"
 
 namespace {
 
@@ -289,6 +290,8 @@ const char* afa_strerror(int code) {
 
 const char* afa_status_string(int32_t status) {
   if (status == AFA_DEV_OK) return "ok";
+  if (status == AFA_DEV_BAD_PAGE) return "cache: a page_table entry in use is not a page of the cache";
+  if (status == AFA_DEV_BAD_LENGTH) return "cache: a sequence's kv_lens or new_lens is negative or too large";
   switch (status - AFA_DEV_TIMEOUT_BASE) {
     case afa100::kSiteLoadQEmpty: return "timeout: TMA producer waiting for a free Q buffer";
     case afa100::kSiteLoadKVEmpty: return "timeout: TMA producer waiting for a free K/V slot";

@@ -42,12 +42,14 @@
 #include <vector>
 
 #include "afa_sm100.h"
+#include "afa_torch_common.h"
+
+using afa_torch::dtype_code;
+using afa_torch::raise_earlier_abort;
+using afa_torch::status_word;
+using afa_torch::take_status;
 
 namespace {
-
-#define AFA_CHECK_CUDA(x) TORCH_CHECK((x).device().is_cuda(), #x " must be a CUDA tensor")
-#define AFA_CHECK_LAST_DIM(x) \
-  TORCH_CHECK((x).dim() == 4 && (x).stride(3) == 1, #x " must be 4-D [batch, seq, heads, head_dim] with a contiguous head_dim")
 
 // The key fields of the Python AFAForwardKernelConfig.  All 13 attributes are
 // read, as in py_to_cpp_kernel_config (csrc/ampere_flash_attention.cu:16-33),
@@ -68,26 +70,18 @@ KernelKey py_to_cpp_kernel_config(const py::object& cfg) {
   return key;
 }
 
+std::mutex g_status_mu;
+std::map<int, afa_torch::StatusWord> g_status;
+
+}  // namespace
+
+namespace afa_torch {
+
 int dtype_code(const at::Tensor& t) {
   if (t.scalar_type() == at::kHalf) return AFA_DTYPE_FP16;
   if (t.scalar_type() == at::kBFloat16) return AFA_DTYPE_BF16;
   return -1;
 }
-
-// One status word per device (int32, zero = ok) in mapped page-locked host
-// memory: every launch on the device gets its device address, a kernel whose
-// bounded wait runs out stores its code there, and the host reads it without
-// synchronising.  Each call first takes (and clears) what earlier launches on
-// its device reported, so a device-side abort is raised by the next call on
-// that device -- at the latest by the first one made after the aborted launch
-// has finished -- or by check_status(), which synchronises first.  Kept until
-// the process exits (4 bytes of page-locked memory per device).
-struct StatusWord {
-  int32_t* host = nullptr;    // what the host reads
-  int32_t* device = nullptr;  // the same word as the kernel addresses it
-};
-std::mutex g_status_mu;
-std::map<int, StatusWord> g_status;
 
 StatusWord status_word(int dev) {
   std::lock_guard<std::mutex> lock(g_status_mu);
@@ -108,16 +102,18 @@ StatusWord status_word(int dev) {
   return w;
 }
 
-// Takes the code earlier launches on `dev` left in the status word and clears it.
 int32_t take_status(int dev) {
   return __atomic_exchange_n(status_word(dev).host, 0, __ATOMIC_ACQ_REL);
 }
 
-// Raises for an abort that a launch made before this call reported.
 void raise_earlier_abort(int dev) {
   const int32_t st = take_status(dev);
   TORCH_CHECK(st == 0, "attention kernel reported (an earlier launch on cuda:", dev, "): ", afa_status_string(st));
 }
+
+}  // namespace afa_torch
+
+namespace {
 
 // Scheduler words of the causal kernel (AfaFwdArgs.sched), one pair per
 // (device, stream) so launches that may overlap never share them; zero at rest
@@ -518,4 +514,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Test hook: AFA_TEST_* flags and wait bound for the next launch only");
   m.def("_raise_formatted_error", &raise_formatted_error, py::arg("a"), py::arg("b"));
   m.def("kernel_keys", &kernel_keys, "(dtype code, d_head) pairs with a compiled sm_100a kernel");
+  afa_torch::bind_ops(m);
 }

@@ -1,0 +1,138 @@
+// ops_common.cuh -- what the launchers and kernels of the cache operators and
+// of the rotary positions (include/afa_sm100_ops.h) share.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <mutex>
+
+#include "afa_sm100_ops.h"
+
+namespace afa100 {
+
+constexpr int kOpsMaxDevices = 64;
+
+// Current device, its SM count and that it is compute capability 10.0; probed
+// once per device.
+inline int ops_device(int* dev_out, int* sm_count_out) {
+  static std::mutex mu;
+  static int sms[kOpsMaxDevices] = {};  // 0: not probed, -1: another architecture
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kOpsMaxDevices) {
+    cudaGetLastError();
+    return AFA_ERR_NO_DEVICE;
+  }
+  std::lock_guard<std::mutex> lock(mu);
+  if (sms[dev] == 0) {
+    int major = 0, minor = 0, n = 0;
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+      cudaGetLastError();
+      return AFA_ERR_NO_DEVICE;
+    }
+    sms[dev] = major == 10 && minor == 0 ? n : -1;
+  }
+  if (sms[dev] < 0) return AFA_ERR_ARCH;
+  *dev_out = dev;
+  *sm_count_out = sms[dev];
+  return AFA_OK;
+}
+
+inline int ops_launched() {
+  if (cudaGetLastError() != cudaSuccess) return AFA_ERR_LAUNCH;
+  return AFA_OK;
+}
+
+inline bool ops_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0u; }
+
+// Strides (batch, seq, head) of a 16-bit tensor whose rows are moved 16 bytes
+// at a time; a stride of a size-1 dimension is never used.  Inputs may repeat
+// (stride 0), outputs may not.
+inline bool ops_strides_ok(const int64_t s[3], int64_t batch, int64_t seq, int64_t heads, bool output) {
+  const int64_t ext[3] = {batch, seq, heads};
+  for (int i = 0; i < 3; ++i)
+    if (ext[i] > 1 && (s[i] % 8 != 0 || s[i] < (output ? 8 : 0))) return false;
+  return true;
+}
+
+// Two 16-bit values of a 32-bit word as fp32 and back.
+template <bool kBF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (kBF16) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  }
+}
+template <bool kBF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (kBF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+__device__ __forceinline__ uint4 ldg_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+// The kernels' report of a bad table entry or length (include/afa_sm100_ops.h).
+__device__ __forceinline__ void report(int32_t* status, int32_t code) {
+  if (status != nullptr) *static_cast<volatile int32_t*>(status) = code;
+}
+
+// A sequence's lengths as the cache kernels use them: new rows and the position
+// of row 0, or no rows at all (reported) where they contradict each other.
+struct NewRows {
+  int count;
+  int first;
+};
+__device__ __forceinline__ NewRows new_rows(const AfaCache4& c, int b, int seq_len) {
+  const int kv = c.kv_lens[b];
+  const int fresh = c.new_lens != nullptr ? c.new_lens[b] : seq_len;
+  if (kv < 0 || static_cast<int64_t>(kv) > static_cast<int64_t>(c.max_pages) * c.page_size || fresh < 0 ||
+      fresh > seq_len || fresh > kv) {
+    report(c.status, AFA_DEV_BAD_LENGTH);
+    return NewRows{0, 0};
+  }
+  return NewRows{fresh, kv - fresh};
+}
+
+inline int ops_log2(int v) {
+  int s = 0;
+  while ((1 << s) < v) ++s;
+  return s;
+}
+
+// The cache argument's own checks, shared by the three cache operators.
+inline int ops_check_cache(const AfaCache4* c) {
+  if (c == nullptr) return AFA_ERR_INVALID_ARGUMENT;
+  if (c->dtype != AFA_DTYPE_FP16 && c->dtype != AFA_DTYPE_BF16) return AFA_ERR_UNSUPPORTED_DTYPE;
+  if (c->head_dim != 64 && c->head_dim != 128) return AFA_ERR_NO_KERNEL;
+  if (c->cache == nullptr || c->page_table == nullptr || c->kv_lens == nullptr) return AFA_ERR_INVALID_ARGUMENT;
+  if (c->n_pages <= 0 || c->max_pages <= 0 || c->batch <= 0 || c->n_kv_heads <= 0) return AFA_ERR_INVALID_ARGUMENT;
+  if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)) != 0)
+    return AFA_ERR_INVALID_ARGUMENT;
+  if (!ops_aligned16(c->cache) || c->page_stride % 16 != 0) return AFA_ERR_MISALIGNED;
+  if ((reinterpret_cast<uintptr_t>(c->page_table) & 3u) != 0u || (reinterpret_cast<uintptr_t>(c->kv_lens) & 3u) != 0u ||
+      (reinterpret_cast<uintptr_t>(c->new_lens) & 3u) != 0u || (reinterpret_cast<uintptr_t>(c->status) & 3u) != 0u)
+    return AFA_ERR_MISALIGNED;
+  const int64_t page_bytes = int64_t{2} * c->n_kv_heads * c->page_size * afa_cache4_row_bytes(c->head_dim);
+  if (c->n_pages > 1 && c->page_stride < page_bytes) return AFA_ERR_INVALID_ARGUMENT;
+  if (c->batch > 1 && c->table_stride < 0) return AFA_ERR_INVALID_ARGUMENT;
+  if (int64_t{1} * c->max_pages * c->page_size > INT32_MAX - 512) return AFA_ERR_TOO_LARGE;
+  return AFA_OK;
+}
+
+}  // namespace afa100

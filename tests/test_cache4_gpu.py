@@ -1,0 +1,563 @@
+"""The paged 4-bit cache on the GPU: the writer's bytes against exact arithmetic,
+the reader's values, and attention over the cache against a 64-bit oracle.
+
+Tolerances.
+* Writer: none; codes, steps and minima are equal.
+* Reader: s c + m rounded once: half a step of the value's type.
+* Attention: with p the weights of a row, the output is rounded once (eps / 2
+  relative) from sum_t p_t (s' c' + m'), where p s' was rounded to fp16 (2^-11
+  relative) and each p is off by twice its score's error and that of the base-2
+  exponential (2^-21).  A score is a sum of at most 8 matrix instructions and 6
+  fp32 steps over terms that add up to `reach` in magnitude; each is charged a
+  whole unit of the 23rd bit: 14 * 2^-23 < 2^-19 reach.  l and the sums over the
+  tokens add below 2^-16 (at most 2^12 fp32 additions a lane, each half a unit of the
+  24th bit).  So
+      |O - O64| <= eps / 2 |O64| + (2^-11 + 2^-18 reach + 2^-15) weight
+  with weight = sum_t p_t (s' c' + |m'|), and
+      |lse - lse64| <= 2^-19 reach + 2^-15 + 2^-22 |lse64|.
+"""
+
+import math
+
+import pytest
+import torch
+
+import afa_flash_attention_kernels as fa
+from oracle import cache4_oracle as oc
+
+pytestmark = pytest.mark.gpu
+
+TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}
+
+
+def pages(lens, page, seed=0, spare=2):
+    """Page table (-1 behind a sequence's last page) over shuffled pages, on the CPU."""
+    need = [max(1, -(-n // page)) for n in lens]
+    order = torch.randperm(sum(need) + spare, generator=torch.Generator().manual_seed(seed)).int()
+    table = torch.full((len(lens), max(need)), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        at += n
+    return table, sum(need) + spare
+
+
+def noise_cache(n_pages, heads, page, d, seed=0):
+    """Pages that hold anything, NaN and infinite steps among it."""
+    g = torch.Generator().manual_seed(seed)
+    c = torch.randint(0, 256, (n_pages, heads, 2, page, d // 2 + d // 16), generator=g, dtype=torch.uint8)
+    c[:, :, :, ::3, d // 2:] = 255
+    return c
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def filled(lens, heads, d, page, dtype, seed=0, k_scale=1.0, v_scale=1.0, offset=1.0):
+    """(cache, table) on the CPU with every sequence's tokens quantised by the oracle; other rows are noise."""
+    table, n_pages = pages(lens, page, seed)
+    cache = noise_cache(n_pages, heads, page, d, seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    for b, n in enumerate(lens):
+        if n == 0:
+            continue
+        t = torch.arange(n)
+        for w, scale in ((0, k_scale), (1, v_scale)):
+            x = torch.randn(n, heads, d, generator=g) * scale
+            if w == 0:
+                x += offset * torch.randn(heads, d, generator=g)
+            rows = oc.pack_rows(*oc.quantise64(x.to(dtype), dtype), dtype)
+            cache[table[b, t // page].long(), :, w, t % page] = rows
+    return cache, table
+
+
+# --- writer ----------------------------------------------------------------------------------------------
+def hard_rows(dtype, d, seed):
+    """Rows where rounding is decided close: halves, constants, far ranges, tiny and large values."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(96, d, generator=g)
+    x[0] = 0
+    x[1] = -3.5
+    x[2] = torch.arange(d) % 31 / 2.0  # range 15: halves of a step
+    x[3] = torch.arange(d) % 16 * 0.25 - 1
+    x[4] = 1e-7 * x[4]
+    x[5] = 1e4 * x[5]
+    x[6, ::2] *= 1e-5
+    x[7] = x[7] * 1e-3 + 100
+    x[8] = (torch.arange(d) % 4) * 2.0 ** -24  # fp16: subnormal steps, a step of 0
+    x[9] = (torch.arange(d) % 64) * 2.0 ** -24
+    x[10, 1:] = 0
+    x[11:40] = torch.randint(-8, 9, (29, d), generator=g) / 4.0  # few bits: many exact ties
+    x[40:60] = torch.randint(0, 200, (20, d), generator=g).float()
+    y = x.to(dtype)
+    if dtype == torch.bfloat16:
+        y[60] = y[60] * 1e37
+        y[61] = (y[61].double() * 1e-39).to(dtype)
+        y[62, 0], y[62, 1] = 3e38, -1e-30
+        y[63, 0], y[63, 1] = -6.5, 1e-30  # next to a border of the step 1
+        y[63, 2] = 8.5
+    return y
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_written_bytes_are_exact(dtype, d):
+    x = hard_rows(dtype, d, 1).view(1, 96, 1, d)
+    table, n_pages = pages([96], 32)
+    cache = noise_cache(n_pages, 1, 32, d).cuda()
+    fa.cache4_write(x.cuda(), x.flip(1).cuda(), cache, table.cuda(), ints([96]).cuda())
+    fa.check_status(0)
+    rows = oc.sequence_rows(cache.cpu(), table, 0, 96)
+    want = oc.quantise_exact(x[0, :, 0], dtype)
+    for got, exp in ((rows[0, :, 0], want), (rows[1, :, 0], tuple(t.flip(0) for t in want))):
+        for a, b, what in zip(oc.unpack_rows(got, dtype), exp, ("codes", "s", "m")):
+            assert torch.equal(a, b), (what, (a != b).nonzero()[:5].tolist())
+
+
+WRITES = [
+    # lens after the write, n, new_lens, heads, d, page, dtype
+    ([1], 1, None, 1, 64, 16, torch.float16),
+    ([1, 500, 64, 65], 1, None, 8, 128, 64, torch.bfloat16),
+    ([300, 257, 1000], 257, None, 3, 64, 128, torch.bfloat16),
+    ([40, 7, 128, 129], 40, [40, 7, 0, 1], 2, 128, 16, torch.float16),
+    ([1300], 1200, None, 5, 128, 256, torch.float16),
+    ([0, 30], 9, [0, 5], 1, 64, 32, torch.bfloat16),
+]
+
+
+@pytest.mark.parametrize("case", WRITES, ids=lambda c: f"n{c[1]}-h{c[3]}-d{c[4]}-p{c[5]}")
+def test_write_and_read_back(case):
+    lens, n, new, heads, d, page, dtype = case
+    B = len(lens)
+    g = torch.Generator().manual_seed(n)
+    k, v = (torch.randn(B, n, heads, d, generator=g).to(dtype) for _ in range(2))
+    table, n_pages = pages(lens, page, n)
+    before = noise_cache(n_pages, heads, page, d)
+    cache = before.cuda()
+    dev = [t.cuda() if t is not None else None for t in (table, ints(lens), ints(new) if new else None)]
+    for t in (k, v):  # padding rows may hold anything
+        for b in range(B):
+            t[b, (new[b] if new else n):] = math.nan
+    fa.cache4_write(k.cuda(), v.cuda(), cache, dev[0], dev[1], dev[2])
+    expect = before.clone()
+    for b in range(B):
+        m = new[b] if new else n
+        for i in range(m):
+            t = lens[b] - m + i
+            for w, x in ((0, k), (1, v)):
+                expect[table[b, t // page], :, w, t % page] = oc.pack_rows(*oc.quantise64(x[b, i], dtype), dtype)
+    assert torch.equal(cache.cpu(), expect)  # the new rows, and nothing else
+    kr, vr = fa.cache4_read(cache, dev[0], dev[1], n, dtype, dev[2])
+    fa.check_status(0)
+    for b in range(B):
+        m = new[b] if new else n
+        rows = oc.sequence_rows(expect, table, b, lens[b])[:, lens[b] - m:]
+        for got, r in ((kr, rows[0]), (vr, rows[1])):
+            c, s, mn = oc.unpack_rows(r, dtype)
+            want = c * s.repeat_interleave(64, -1) + mn.repeat_interleave(64, -1)
+            x = got[b, :m].cpu().double()
+            # rounding once leaves half a step of the value's own binade; |x| covers a value rounded up to a power of two
+            assert torch.all((x - want).abs() <= torch.finfo(dtype).eps / 2 * x.abs() + TINY[dtype])
+            assert not got[b, m:].any()
+
+
+def test_non_finite_groups_read_back_as_nan():
+    x = torch.randn(1, 6, 1, 128, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    x[0, 0, 0, 5] = math.nan
+    x[0, 1, 0, 70] = math.inf
+    x[0, 2, 0, 0] = -math.inf
+    x[0, 3, 0, 64], x[0, 3, 0, 65] = 3e38, -3e38  # the range passes fp32
+    table, lens = ints([[1]]).cuda(), ints([6]).cuda()
+    cache = torch.zeros(2, 1, 2, 16, 72, dtype=torch.uint8, device="cuda")
+    fa.cache4_write(x.cuda(), x.cuda(), cache, table, lens)
+    k, v = fa.cache4_read(cache, table, lens, 6, torch.bfloat16)
+    bad = torch.zeros(6, 2, dtype=torch.bool)
+    bad[0, 0] = bad[1, 1] = bad[2, 0] = bad[3, 1] = True
+    for t in (k, v):
+        nan = torch.isnan(t[0, :, 0].cpu().view(6, 2, 64))
+        assert torch.equal(nan.all(-1), bad) and torch.equal(nan.any(-1), bad)
+
+
+def test_strided_inputs_outputs_and_pages():
+    g = torch.Generator().manual_seed(3)
+    kv = torch.randn(2, 50, 2, 3, 64, generator=g).half().cuda()  # packed keys and values
+    layers = torch.zeros(12, 4, 3, 2, 16, 36, dtype=torch.uint8, device="cuda")  # pages of four layers side by side
+    table = ints([[0, 3, 5, 7, -1], [11, 2, 1, 9, -1]]).cuda()[:, :4]
+    lens = ints([50, 50]).cuda()
+    dense = torch.zeros(12, 3, 2, 16, 36, dtype=torch.uint8, device="cuda")
+    fa.cache4_write(kv[:, :, 0], kv[:, :, 1], layers[:, 2], table, lens)
+    fa.cache4_write(kv[:, :, 0].contiguous(), kv[:, :, 1].contiguous(), dense, table, lens)
+    assert torch.equal(layers[:, 2], dense) and not layers[:, [0, 1, 3]].any()
+    out = torch.full((2, 50, 2, 3, 64), 7.0, dtype=torch.float16, device="cuda")
+    k, v = fa.cache4_read(dense, table, lens, 50, torch.float16)
+    a, b = fa.cache4_read(layers[:, 2], table, lens, 50, torch.float16, None, out[:, :, 0], out[:, :, 1])
+    assert a.data_ptr() == out.data_ptr() and torch.equal(a, k) and torch.equal(b, v)
+    # one row repeated over the batch
+    rep = kv[:1, :, 0].expand(2, 50, 3, 64)
+    fa.cache4_write(rep, rep, dense, table, lens)
+    k, v = fa.cache4_read(dense, table, lens, 50, torch.float16)
+    assert torch.equal(k[0], k[1]) and torch.equal(k, v)
+    q = torch.randn(2, 2, 6, 64, generator=g).half().cuda()
+    fa.cache4_write(kv[:, :, 0], kv[:, :, 1], dense, table, lens)
+    o, lse = fa.forward_cache4(q, dense, table, lens, None, True, None, True)
+    o2, lse2 = fa.forward_cache4(q, layers[:, 2], table, lens, None, True, None, True)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    wide = torch.zeros(2, 6, 2, 2, 64, dtype=torch.float16, device="cuda")  # head-major q, strided o
+    qh = q.transpose(1, 2).contiguous().transpose(1, 2)
+    view = wide[:, :, :, 1].transpose(1, 2)
+    o3, _ = fa.forward_cache4(qh, dense, table, lens, view, True)
+    assert o3.data_ptr() == view.data_ptr() and torch.equal(o3, o) and not wide[:, :, :, 0].any()
+
+
+# --- attention -------------------------------------------------------------------------------------------
+def check_attention(q, cache, table, lens, causal, new=None, scale=None, got=None):
+    B, N = q.shape[:2]
+    if got is None:
+        got = fa.forward_cache4(q.cuda(), cache.cuda(), table.cuda(), ints(lens).cuda(), None, causal, scale, True,
+                                ints(new).cuda() if new else None)
+        fa.check_status(0)
+    o, lse = (t.cpu().double() for t in got)
+    want, want_lse, weight, reach = oc.attention64(q, cache, table, lens, causal, scale, new)
+    eps = torch.finfo(q.dtype).eps
+    tol = want.abs() * eps / 2 + (2.0 ** -11 + 2.0 ** -18 * reach[..., None] + 2.0 ** -15) * weight + TINY[q.dtype]
+    err = (o - want).abs()
+    assert torch.all(err <= tol), f"largest error over tolerance {(err / tol).max().item():.3f}"
+    fin = torch.isfinite(want_lse)
+    assert torch.equal(torch.isfinite(lse), fin) and torch.all(lse[~fin] == -math.inf)
+    tol = 2.0 ** -19 * reach.transpose(1, 2) + 2.0 ** -15 + 2.0 ** -22 * want_lse.abs()
+    assert torch.all(((lse - want_lse).abs() <= tol)[fin])
+    return o, lse
+
+
+ATTEND = [
+    # lens, n, new_lens, H, HK, d, page, causal, dtype
+    ([1], 1, None, 1, 1, 64, 16, False, torch.float16),
+    ([1], 1, None, 8, 1, 128, 64, True, torch.bfloat16),
+    ([15, 16, 17, 31, 32, 33], 1, None, 4, 4, 64, 16, False, torch.bfloat16),
+    ([127, 128, 129, 0, 500], 1, None, 8, 2, 128, 32, False, torch.float16),
+    ([0, 0], 2, None, 2, 1, 64, 16, True, torch.float16),
+    ([1000, 3, 257], 1, None, 32, 8, 128, 64, False, torch.bfloat16),
+    ([700], 1, None, 7, 1, 128, 128, False, torch.float16),
+    ([300, 40], 5, None, 8, 2, 128, 16, True, torch.bfloat16),
+    ([300, 40], 5, None, 8, 2, 64, 256, False, torch.float16),
+    ([64, 3, 90], 7, [7, 3, 1], 6, 3, 64, 32, True, torch.bfloat16),
+    ([64, 0, 90], 7, [7, 0, 0], 6, 3, 128, 32, False, torch.float16),
+    ([2, 1], 4, None, 2, 2, 64, 16, True, torch.float16),  # fewer tokens than rows: rows that see none
+    ([130], 33, None, 4, 2, 128, 64, True, torch.float16),  # several row blocks
+    ([4100], 1, None, 2, 2, 64, 128, False, torch.bfloat16),
+]
+
+
+@pytest.mark.parametrize("case", ATTEND, ids=lambda c: f"{c[0][0]}x{len(c[0])}-n{c[1]}-h{c[3]}.{c[4]}-d{c[5]}-p{c[6]}")
+def test_attention_against_oracle(case):
+    lens, n, new, H, HK, d, page, causal, dtype = case
+    cache, table = filled(lens, HK, d, page, dtype, seed=sum(lens) + n)
+    q = torch.randn(len(lens), n, H, d, generator=torch.Generator().manual_seed(n)).to(dtype)
+    o, lse = check_attention(q, cache, table, lens, causal, new)
+    for b in range(len(lens)):
+        for i in range(n):
+            if i >= (new[b] if new else n) or lens[b] == 0:
+                assert not o[b, i].any() and torch.all(lse[b, :, i] == -math.inf)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_random_shapes(d, dtype):
+    g = torch.Generator().manual_seed(d + (dtype == torch.float16))
+    r = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))
+    for trial in range(12):
+        B, n, HK = r(1, 5), r(1, 6), r(1, 4)
+        H = HK * r(1, 9)
+        lens = [r(0, 900) for _ in range(B)]
+        new = [r(0, n) for _ in range(B)] if r(0, 1) else None
+        page = 16 << r(0, 4)
+        cache, table = filled(lens, HK, d, page, dtype, seed=trial)
+        q = torch.randn(B, n, H, d, generator=g).to(dtype)
+        check_attention(q, cache, table, lens, bool(r(0, 1)), new)
+
+
+@pytest.mark.parametrize("k_scale,v_scale,q_scale", [(8.0, 1.0, 3.0), (1e-3, 1e-4, 1.0), (1.0, 200.0, 30.0), (30.0, 1.0, 1e-3)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_ranges(dtype, k_scale, v_scale, q_scale):
+    lens = [513, 70]
+    cache, table = filled(lens, 2, 128, 32, dtype, seed=5, k_scale=k_scale, v_scale=v_scale)
+    q = (torch.randn(2, 2, 4, 128, generator=torch.Generator().manual_seed(9)) * q_scale).to(dtype)
+    check_attention(q, cache, table, lens, True)
+
+
+def test_rising_maximum_and_steps():
+    # scores and values' steps that grow along the sequence: the references move on every step
+    lens, d, page = [640], 64, 64
+    table, n_pages = pages(lens, page, 1)
+    cache = noise_cache(n_pages, 1, page, d)
+    g = torch.Generator().manual_seed(2)
+    u = torch.randn(d, generator=g)
+    t = torch.arange(640)
+    k = (u * t[:, None] * 0.02 + 0.1 * torch.randn(640, d, generator=g)).half()
+    v = (torch.randn(640, d, generator=g) * 2.0 ** (t[:, None] / 64.0 - 5)).half()
+    for w, x in ((0, k), (1, v)):
+        cache[table[0, t // page].long(), 0, w, t % page] = oc.pack_rows(*oc.quantise64(x, torch.float16), torch.float16)
+    q = torch.stack([u, -u, 0 * u]).half().view(1, 1, 3, d)
+    check_attention(q, cache, table, lens, False)
+
+
+def test_softmax_scale_and_lse_optional():
+    cache, table = filled([100], 1, 64, 16, torch.float16)
+    q = torch.randn(1, 1, 2, 64, generator=torch.Generator().manual_seed(1)).half()
+    check_attention(q, cache, table, [100], False, scale=0.3)
+    dev = (q.cuda(), cache.cuda(), table.cuda(), ints([100]).cuda())
+    o, none = fa.forward_cache4(*dev)
+    assert none is None and torch.equal(o, fa.forward_cache4(*dev, return_lse=True)[0])
+
+
+def test_nan_in_masked_places_stays_there():
+    # NaN keys and values behind a row's position must not reach it; a visible one must
+    lens, n = [50], 4
+    cache, table = filled(lens, 1, 128, 16, torch.float16, seed=3)
+    q = torch.randn(1, n, 2, 128, generator=torch.Generator().manual_seed(1)).half()
+    clean, _ = check_attention(q, cache, table, lens, True)
+    for side in (0, 1):
+        bad = cache.clone()
+        bad[table[0, 48 // 16], 0, side, 48 % 16, 64:] = 255  # token 48: rows 2 and 3 see it
+        o, _ = fa.forward_cache4(q.cuda(), bad.cuda(), table.cuda(), ints(lens).cuda(), None, True)
+        fa.check_status(0)
+        assert torch.equal(o[:, :2].cpu().double(), clean[:, :2])
+        assert torch.isnan(o[:, 2:]).all()
+
+
+def test_negative_steps_are_taken_as_written():
+    # the format allows any s; rows from elsewhere may hold negative ones
+    cache, table = filled([40], 1, 64, 16, torch.float16, seed=6)
+    c, s, m = oc.unpack_rows(cache, torch.float16)
+    s = torch.where(torch.isfinite(s), s, torch.ones_like(s))
+    m = torch.where(torch.isfinite(m), m, torch.ones_like(m))
+    flipped = oc.pack_rows(15 - c, -s, m + 15 * s, torch.float16)
+    q = torch.randn(1, 1, 1, 64, generator=torch.Generator().manual_seed(1)).half()
+    _, fs, fm = oc.unpack_rows(oc.sequence_rows(flipped, table, 0, 40), torch.float16)
+    want, want_lse, _, _ = oc.attention64(q, flipped, table, [40])
+    o, lse = fa.forward_cache4(q.cuda(), flipped.cuda(), table.cuda(), ints([40]).cuda(), return_lse=True)
+    # terms s c and m of either sign: their magnitudes bound both errors (as above)
+    size = float((15 * fs.abs() + fm.abs()).max())
+    reach = float(q.double().abs().sum()) * size / 8
+    assert torch.all((o.cpu().double() - want).abs() <= want.abs() * 2.0 ** -11 + size * (2.0 ** -11 + 2.0 ** -18 * reach + 2.0 ** -15))
+    assert abs(lse.item() - want_lse.item()) <= 2.0 ** -19 * reach + 2.0 ** -15 + 2.0 ** -22 * abs(want_lse.item())
+
+
+# --- lengths and pages that are wrong --------------------------------------------------------------------
+@pytest.mark.parametrize("entry", ["write", "read", "attend"])
+@pytest.mark.parametrize("fault", ["page low", "page high", "length high", "length low", "new high", "new low"])
+def test_bad_tables_and_lengths_are_reported(entry, fault):
+    table, lens, new = ints([[0, 1], [2, 3]]), ints([20, 30]), ints([2, 2])
+    if fault == "page low":
+        table[1, 1] = -1
+    elif fault == "page high":
+        table[1, 1] = 4
+    elif fault == "length high":
+        lens[1] = 33
+    elif fault == "length low":
+        lens[1] = -1
+    elif fault == "new high":
+        new[1] = 3
+    else:
+        new[1] = -1
+    cache = torch.zeros(4, 1, 2, 16, 36, dtype=torch.uint8, device="cuda")
+    x = torch.ones(2, 2, 1, 64, dtype=torch.float16, device="cuda")
+    table, lens, new = table.cuda(), lens.cuda(), new.cuda()
+    fa.check_status(0)
+    if entry == "write":
+        fa.cache4_write(x, x, cache, table, lens, new)
+    elif entry == "read":
+        fa.cache4_read(cache, table, lens, 2, torch.float16, new)
+    else:
+        fa.forward_cache4(x, cache, table, lens, new_lens=new)
+    torch.cuda.synchronize()
+    want = "page_table" if fault.startswith("page") else "kv_lens"
+    with pytest.raises(RuntimeError, match=f"earlier launch on cuda:0.*{want}"):
+        fa.forward_cache4(x, cache, ints([[0, 1], [2, 3]]).cuda(), ints([20, 30]).cuda())
+    fa.check_status(0)  # raised once
+    if entry == "write":  # the other sequence's rows were written, no others
+        used = cache.flatten(1).any(-1).tolist()
+        assert used == [False, True, False, False]
+
+
+def test_new_rows_beyond_the_sequence_are_refused_by_the_movers():
+    # a sequence shorter than the rows to write has no place for them; attention allows it (rows that see nothing)
+    cache = torch.zeros(2, 1, 2, 16, 36, dtype=torch.uint8, device="cuda")
+    x = torch.ones(1, 3, 1, 64, dtype=torch.float16, device="cuda")
+    fa.cache4_write(x, x, cache, ints([[0]]).cuda(), ints([2]).cuda())
+    with pytest.raises(RuntimeError, match="kv_lens"):
+        fa.check_status(0)
+    assert not cache.any()
+    fa.forward_cache4(x, cache, ints([[0]]).cuda(), ints([2]).cuda())
+    fa.check_status(0)
+
+
+def test_refusals():
+    cache = torch.zeros(4, 2, 2, 16, 36, dtype=torch.uint8, device="cuda")
+    x = torch.zeros(2, 3, 2, 64, dtype=torch.float16, device="cuda")
+    table, lens = ints([[0, 1], [2, 3]]).cuda(), ints([20, 30]).cuda()
+    w = lambda **o: fa.cache4_write(**{**dict(k=x, v=x, cache=cache, page_table=table, kv_lens=lens), **o})
+    r = lambda **o: fa.cache4_read(**{**dict(cache=cache, page_table=table, kv_lens=lens, n=3, dtype=torch.float16), **o})
+    a = lambda **o: fa.forward_cache4(**{**dict(q=x, cache=cache, page_table=table, kv_lens=lens), **o})
+    shared = [
+        (dict(cache=cache.char()), "uint8"),
+        (dict(cache=cache[..., :20]), "rows of"),
+        (dict(cache=cache[:, :, :, :12]), "page_size"),
+        (dict(cache=cache[:, :, :, ::2][:, :, :, :8]), "page_size"),
+        (dict(cache=torch.zeros(4, 2, 2, 32, 36, dtype=torch.uint8, device="cuda")[:, :, :, ::2]), "dense"),
+        (dict(cache=cache[:0]), "positive"),
+        (dict(cache=cache[:1].expand(4, 2, 2, 16, 36)), "invalid argument"),
+        (dict(page_table=table.long()), "int32"),
+        (dict(page_table=table.t()), "contiguous rows"),
+        (dict(page_table=table[0]), "page_table must be"),
+        (dict(page_table=table.cpu()), "CUDA tensor"),
+        (dict(kv_lens=lens.long()), "int32"),
+        (dict(kv_lens=lens[:1]), "kv_lens must be"),
+        (dict(kv_lens=ints([1, 2, 3, 4]).cuda()[::2]), "kv_lens must be"),
+        (dict(new_lens=lens[:1]), "new_lens must be"),
+        (dict(new_lens=lens.long()), "int32"),
+    ]
+    for fn in (w, r, a):
+        for over, match in shared:
+            with pytest.raises(RuntimeError, match=match):
+                fn(**over)
+    for over, match in [(dict(v=x[:1]), "same shape"), (dict(v=x.bfloat16()), "same data type"), (dict(k=x.float(), v=x.float()), "Only fp16"),
+                        (dict(k=x[:, :, :1], v=x[:, :, :1]), "do not match"), (dict(k=x[..., :32], v=x[..., :32]), "do not match"),
+                        (dict(k=x[:, :0], v=x[:, :0]), "positive"), (dict(k=x.transpose(2, 3)), "contiguous"), (dict(k=x.cpu()), "CUDA tensor")]:
+        with pytest.raises(RuntimeError, match=match):
+            w(**over)
+    for over, match in [(dict(n=0), "n must be"), (dict(dtype=torch.float32), "Only fp16"), (dict(k_out=x[:, :2]), "k_out must be"),
+                        (dict(v_out=x.bfloat16()), "v_out must be")]:
+        with pytest.raises(RuntimeError, match=match):
+            r(**over)
+    for over, match in [(dict(q=x[:, :, :1]), "multiple of"), (dict(q=x.float()), "Only fp16"), (dict(q=x[..., :32].contiguous()), "differ"),
+                        (dict(softmax_scale=0.0), "softmax_scale"), (dict(o=x[:1]), "same shape"), (dict(o=x.bfloat16()), "dtype")]:
+        with pytest.raises(RuntimeError, match=match):
+            a(**over)
+    fa.check_status(0)
+
+
+# --- streams, graphs, several calls ----------------------------------------------------------------------
+def test_captured_steps_follow_their_inputs():
+    # a decode step (write, attend) captured once and replayed as the sequences grow; two graphs side by side
+    d, page, heads = 128, 16, 2
+    graphs = []
+    for i in range(2):
+        table = torch.arange(8, dtype=torch.int32).view(2, 4).cuda()
+        cache = torch.zeros(8, heads, 2, page, 72, dtype=torch.uint8, device="cuda")
+        k, v = (torch.zeros(2, 1, heads, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        q = torch.zeros(2, 1, 4 * heads, d, dtype=torch.bfloat16, device="cuda")
+        lens = ints([1, 1]).cuda()
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            fa.cache4_write(k, v, cache, table, lens)
+            fa.forward_cache4(q, cache, table, lens, return_lse=True)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            fa.cache4_write(k, v, cache, table, lens)
+            o, lse = fa.forward_cache4(q, cache, table, lens, return_lse=True)
+        graphs.append((graph, stream, k, v, q, lens, cache, table, o, lse))
+    g = torch.Generator().manual_seed(1)
+    for step in range(1, 60):
+        for graph, stream, k, v, q, lens, *_ in graphs:
+            for t in (k, v, q):
+                t.copy_(torch.randn(t.shape, generator=g))
+            lens.copy_(ints([step, max(1, step - 20)]))
+        torch.cuda.synchronize()
+        for graph, stream, *_ in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        if step % 13 == 0:
+            for _, _, k, v, q, lens, cache, table, o, lse in graphs:
+                check_attention(q.cpu(), cache.cpu(), table.cpu(), lens.tolist(), False, got=(o, lse))
+    fa.check_status(0)
+
+
+def test_calls_at_once_on_two_streams_agree_with_one():
+    lens = [900, 1300, 5, 0]
+    cache, table = filled(lens, 2, 128, 32, torch.float16, seed=4)
+    cache, table, lens = cache.cuda(), table.cuda(), ints(lens).cuda()
+    qs = [torch.randn(4, 3, 8, 128, generator=torch.Generator().manual_seed(i)).half().cuda() for i in range(2)]
+    want = [fa.forward_cache4(q, cache, table, lens, None, True, None, True) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    for _ in range(20):
+        got = []
+        for q, s in zip(qs, streams):
+            with torch.cuda.stream(s):
+                got.append(fa.forward_cache4(q, cache, table, lens, None, True, None, True))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        del got
+    fa.check_status(0)
+
+
+def test_result_does_not_depend_on_other_sequences_beyond_rounding():
+    # the same sequence alone and in a ragged batch: the split differs, both hold to the oracle
+    lens = [2000, 1, 777, 128, 3000, 64]
+    cache, table = filled(lens, 1, 64, 64, torch.float16, seed=8)
+    q = torch.randn(6, 1, 4, 64, generator=torch.Generator().manual_seed(2)).half()
+    check_attention(q, cache, table, lens, False)
+    check_attention(q[2:3], cache, table[2:3], lens[2:3], False)
+
+
+def test_far_pages_pass_32_bit_offsets():
+    # a pool of 5 GB: rows near its end are written, read and attended to
+    n_pages = 5 * 2 ** 30 // (8 * 2 * 128 * 72)
+    cache = torch.empty(n_pages, 8, 2, 128, 72, dtype=torch.uint8, device="cuda")
+    assert cache.numel() > 2 ** 32
+    table = ints([[n_pages - 1, n_pages - 2], [0, n_pages // 2]]).cuda()
+    lens = ints([200, 200]).cuda()
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(2, 200, 8, 128, generator=g).half() for _ in range(2))
+    fa.cache4_write(k.cuda(), v.cuda(), cache, table, lens)
+    small = torch.stack([cache[i] for i in table.flatten().tolist()])
+    near = ints([[0, 1], [2, 3]]).cuda()
+    q = torch.randn(2, 1, 16, 128, generator=g).half()
+    o, lse = fa.forward_cache4(q.cuda(), cache, table, lens, return_lse=True)
+    assert all(torch.equal(a, b) for a, b in zip(fa.cache4_read(cache, table, lens, 200, torch.float16),
+                                                 fa.cache4_read(small, near, lens, 200, torch.float16)))
+    check_attention(q, small.cpu(), near.cpu(), [200, 200], False, got=(o, lse))
+    fa.check_status(0)
+
+
+# --- together --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompt_then_tokens(dtype):
+    """Positions, cache and attention as a model uses them: a ragged prompt is turned and written, attended to by
+    forward_ext over the values read back, then tokens follow one and three at a time."""
+    B, H, HK, d, page = 2, 8, 2, 128, 32
+    prompt, g = [50, 81], torch.Generator().manual_seed(7)
+    inv = (10000.0 ** (-torch.arange(64, dtype=torch.float64) / 64)).float().cuda()
+    table, n_pages = pages([200, 200], page, 3)
+    cache = noise_cache(n_pages, HK, page, d).cuda()
+    table = table.cuda()
+    made = lambda n, h: torch.randn(B, n, h, d, generator=g).to(dtype).cuda()
+    lens, n = list(prompt), max(prompt)
+    q, k, v = made(n, H), made(n, HK), made(n, HK)
+    pos = torch.arange(n).expand(3, B, n).cuda()
+    q, k = fa.rotary(q, k, pos, inv, [16, 24, 24])
+    fa.cache4_write(k, v, cache, table, ints(lens).cuda(), ints(lens).cuda())
+    kr, vr = fa.cache4_read(cache, table, ints(lens).cuda(), n, dtype, ints(lens).cuda())
+    for b in range(B):
+        m = lens[b]
+        dense, dense_lse = fa.forward_ext(q[b:b + 1, :m], kr[b:b + 1, :m], vr[b:b + 1, :m], None, True, None, True)
+        o, lse = check_attention(q[b:b + 1, :m].cpu(), cache.cpu(), table[b:b + 1].cpu(), [m], True)
+        # forward_ext sees K and V rounded to 16 bits and rounds P to them: its own parity bound against fp32
+        tol = 1e-2 if dtype == torch.float16 else 4e-2
+        assert (dense.cpu().double() - o).abs().max() <= tol
+        assert (dense_lse.cpu().double() - lse).abs().max() <= tol
+    for step in (1, 1, 3, 1):
+        lens = [x + step for x in lens]
+        q, k, v = made(step, H), made(step, HK), made(step, HK)
+        pos = (ints(lens).cuda()[:, None] - step + torch.arange(step).cuda()).expand(3, B, step)
+        q, k = fa.rotary(q, k, pos, inv, [16, 24, 24])
+        fa.cache4_write(k, v, cache, table, ints(lens).cuda())
+        got = fa.forward_cache4(q, cache, table, ints(lens).cuda(), None, True, None, True)
+        check_attention(q.cpu(), cache.cpu(), table.cpu(), lens, True, got=got)
+    fa.check_status(0)
