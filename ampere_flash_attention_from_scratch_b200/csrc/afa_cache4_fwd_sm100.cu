@@ -13,9 +13,9 @@
 //
 //   * q is held in fp16 for either type, each row scaled by a power of two so
 //     that its largest element lies in [2^13, 2^14); the product is exact.
-//   * p s' is rounded to fp16 after a scaling by a power of two a warp keeps for
-//     each group (the largest step so far), at most 2^13: relative 2^-12 as for
-//     a 16-bit P, with 2^-38 of the largest as the smallest step.
+//   * p s' is rounded to fp16: 2^-12 relative, as for a 16-bit P.  A power of two
+//     in the exponent of p keeps the largest product so far below 2^15, which
+//     leaves 2^-31 of it as the smallest that keeps a bit.
 //   * p, its sum, the running maximum and both accumulators are fp32.
 //
 // Bound: HBM for a few query rows -- 1.125 bytes a channel and token for keys
@@ -45,9 +45,10 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStep = 32;               // tokens of a warp's step
 constexpr int kUnit = kWarps * kStep;   // tokens of a unit
-constexpr int kStages = 4;              // steps in flight for a warp
+constexpr int kStages = 4;              // steps of a warp's ring, one less in flight
+constexpr int kItemUnits = 1;           // units an item is charged beside its tokens'
 constexpr float kRescale = 8.0f;        // log2 units a score may pass the reference maximum by
-constexpr float kPScale = 32.0f;        // p s' is at most 2^kRescale * kPScale = 2^13
+constexpr float kHeadroom = 7.0f;       // log2 of p s' at the reference maximum and the largest step
 
 struct FwdParams4 {
   AfaCache4 c;
@@ -61,8 +62,8 @@ struct FwdParams4 {
   int32_t rows;       // seq_len * group query rows of a key/value head
   int32_t row_tiles;  // blocks of kRows of them
   int32_t page_shift;
+  uint32_t page_stride;
   int32_t causal;
-  int32_t min_units;  // units a CTA takes at least
   float scale_log2;
 };
 
@@ -74,16 +75,14 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
+// p + n * stride bytes
+__device__ __forceinline__ const char* far(const char* p, uint32_t n, uint32_t stride) {
+  uint64_t r;
+  asm("mad.wide.u32 %0, %1, %2, %3;" : "=l"(r) : "r"(n), "r"(stride), "l"(reinterpret_cast<uint64_t>(p)));
+  return reinterpret_cast<const char*>(r);
 }
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
+__device__ __forceinline__ uint32_t lds32(const char* a) { return *reinterpret_cast<const uint32_t*>(a); }
+__device__ __forceinline__ uint2 lds64(const char* a) { return *reinterpret_cast<const uint2*>(a); }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -91,9 +90,29 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same from zero: d = a b.
+__device__ __forceinline__ void mma16816_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// With m's bits: the bits of w, or those of 15 - w where x has them too; without
+// them: x.  One three-input operation.
+__device__ __forceinline__ uint32_t pick(uint32_t w, uint32_t m, uint32_t x) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(w), "r"(m), "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) { return pack2<false>(lo, hi); }
@@ -123,36 +142,47 @@ __device__ __forceinline__ int tokens_of(const FwdParams4& p, int b) {
   }
   return kv;
 }
-__device__ __forceinline__ int units_of(int tokens) { return tokens <= kUnit ? 1 : (tokens + kUnit - 1) / kUnit; }
+// Units of an item: kItemUnits that stand for what starting and ending an item
+// costs, then those of its tokens (one at least).
+__device__ __forceinline__ int units_of(int tokens) {
+  return kItemUnits + (tokens <= kUnit ? 1 : (tokens + kUnit - 1) / kUnit);
+}
 
 struct Division {
-  long long total;  // units of the call
-  int ctas;         // CTAs that share them
+  int ctas;  // CTAs that share the units: the first `more` of them take each + 1, the others `each`
+  int each, more;
   // First unit of CTA i.
-  __device__ __forceinline__ long long first(int i) const { return total * i / ctas; }
+  __device__ __forceinline__ int first(int i) const { return i * each + min(i, more); }
+  // The CTA that holds unit u.
+  __device__ __forceinline__ int holder(int u) const {
+    const int longer = more * (each + 1);
+    return u < longer ? u / (each + 1) : more + (u - longer) / each;
+  }
 };
 
 // Sum of units over this lane's share of the sequences, a contiguous range of
-// `per` of them, and from it the division.
-__device__ __forceinline__ Division divide(const FwdParams4& p, int per, long long* before_lane) {
+// `per` of them, and from it the division.  The host has made sure that the
+// units of the call fit 31 bits.
+__device__ __forceinline__ Division divide(const FwdParams4& p, int per, int grid, int* before_lane) {
   const int lane = static_cast<int>(threadIdx.x & 31u);
-  long long mine = 0;
+  int mine = 0;
   for (int i = 0; i < per; ++i) {
     const int b = lane * per + i;
     if (b < p.c.batch) mine += units_of(tokens_of(p, b));
   }
-  mine *= static_cast<long long>(p.c.n_kv_heads) * p.row_tiles;
-  long long upto = mine;
+  mine *= p.c.n_kv_heads * p.row_tiles;
+  int upto = mine;
 #pragma unroll
   for (int i = 1; i < 32; i <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, upto, i);
+    const int v = __shfl_up_sync(0xffffffffu, upto, i);
     if (lane >= i) upto += v;
   }
   *before_lane = upto - mine;
+  const int total = __shfl_sync(0xffffffffu, upto, 31);
   Division d;
-  d.total = __shfl_sync(0xffffffffu, upto, 31);
-  const long long most = (d.total + p.min_units - 1) / p.min_units;
-  d.ctas = static_cast<int>(most < gridDim.x ? most : gridDim.x);
+  d.ctas = min(total, grid);
+  d.each = total / d.ctas;
+  d.more = total - d.each * d.ctas;
   return d;
 }
 
@@ -165,26 +195,53 @@ struct Item {
 };
 
 // The item that unit u belongs to.
-__device__ __forceinline__ Item find_item(const FwdParams4& p, int per, long long before_lane, long long u) {
+__device__ __forceinline__ Item find_item(const FwdParams4& p, int per, int before_lane, int u) {
   const int items = p.c.n_kv_heads * p.row_tiles;
   const unsigned owners = __ballot_sync(0xffffffffu, before_lane <= u);
   const int owner = 31 - __clz(owners);
-  long long left = u - __shfl_sync(0xffffffffu, before_lane, owner);
+  int left = u - __shfl_sync(0xffffffffu, before_lane, owner);
   // lanes behind the last sequence own nothing and start where it ends: u is below that
   Item it;
   it.b = owner * per;
   for (;;) {
     it.tokens = tokens_of(p, it.b);
     it.units = units_of(it.tokens);
-    const long long here = static_cast<long long>(it.units) * items;
+    const int here = it.units * items;
     if (left < here || it.b + 1 >= p.c.batch) break;
     left -= here;
     ++it.b;
   }
-  it.which = static_cast<int>(left / it.units);
-  it.unit = static_cast<int>(left - static_cast<long long>(it.which) * it.units);
+  it.which = left / it.units;
+  it.unit = left - it.which * it.units;
   return it;
 }
+
+// A CTA's walk through its units, piece by piece (a piece: its part of one item).
+struct Walk {
+  Item it;
+  int left;      // units of the CTA from this piece on
+  int unit_end;  // end of the piece within the item
+  int tok, tok_end;
+  __device__ __forceinline__ void open(int warp) {
+    unit_end = it.unit + left < it.units ? it.unit + left : it.units;
+    tok = max(it.unit - kItemUnits, 0) * kUnit + warp * kStep;
+    tok_end = min(it.tokens, max(unit_end - kItemUnits, 0) * kUnit);
+  }
+  // To the next piece; false at the end of the CTA's units.
+  __device__ __forceinline__ bool next(const FwdParams4& p, int warp) {
+    left -= unit_end - it.unit;
+    if (left <= 0) return false;
+    it.unit = 0;
+    if (++it.which == p.c.n_kv_heads * p.row_tiles) {
+      it.which = 0;
+      ++it.b;
+      it.tokens = tokens_of(p, it.b);
+      it.units = units_of(it.tokens);
+    }
+    open(warp);
+    return true;
+  }
+};
 
 // ---------------------------------------------------------------------------
 // Attention
@@ -194,12 +251,15 @@ struct FwdLayout4 {
   static constexpr int kGroups = kD / 64;
   static constexpr int kRow = kD / 2 + kD / 16;
   static constexpr int kRows = kNT * 8;
-  static constexpr int kTileBytes = 16 * kRow;           // 16 tokens of keys or values
-  static constexpr int kStageBytes = 4 * kTileBytes;     // [16 tokens][keys, values]
+  static constexpr int kSideBytes = kStep * kRow;      // keys, or values, of a step
+  static constexpr int kStageBytes = 2 * kSideBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
-  static constexpr int kSmem = kWarps * kWarpBytes + kWarps * kRows * 2 * 4;
-  static constexpr int kShare = kRows * (kD + 2);        // floats of a CTA's share of an item
-  static_assert(kRows * kD * 4 <= kWarpBytes, "a warp's O fits its own stages");
+  static constexpr int kShareBytes = kRows * kD * 4;   // a warp's O
+  // A warp's O fits the stage it has just used, or has memory of its own.
+  static constexpr bool kInStage = kShareBytes <= kStageBytes;
+  static constexpr int kStats = kWarps * (kWarpBytes + (kInStage ? 0 : kShareBytes));
+  static constexpr int kSmem = kStats + kWarps * kRows * 2 * 4 + kWarps * 4;
+  static constexpr int kShare = kRows * (kD + 2);      // floats of a CTA's share of an item
 };
 
 template <int kD, bool kBF16, int kNT>
@@ -211,57 +271,120 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(smem) + warp * L::kWarpBytes;
-  float* stats = reinterpret_cast<float*>(smem + kWarps * L::kWarpBytes);  // [warp][row][m, l]
+  float* stats = reinterpret_cast<float*>(smem + L::kStats);                 // [warp][row][m, l]
+  uint32_t* places = reinterpret_cast<uint32_t*>(stats + kWarps * L::kRows * 2);  // [warp] where its O is
 
-  const int per = (p.c.batch + 31) / 32;
-  long long before_lane;
-  const Division div = divide(p, per, &before_lane);
-  const int cta = blockIdx.x;
-  if (cta >= div.ctas) return;
-  long long u = div.first(cta);
-  const long long u_end = div.first(cta + 1);
-  Item it = find_item(p, per, before_lane, u);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take the SMs as they fall free
+  Walk w;
+  {
+    const int per = (p.c.batch + 31) / 32;
+    int before_lane;
+    const Division div = divide(p, per, gridDim.x, &before_lane);
+    const int cta = static_cast<int>(blockIdx.x);
+    if (cta >= div.ctas) return;
+    w.it = find_item(p, per, before_lane, div.first(cta));
+    w.left = div.first(cta + 1) - div.first(cta);
+    w.open(warp);
+  }
+  // Past pieces that are only the cost of an item whose tokens another CTA has; false at the end.
+  auto skip_empty = [&](Walk& walk) {
+    bool go = true;
+    while (go && walk.unit_end <= kItemUnits) go = walk.next(p, warp);
+    return go;
+  };
 
-  while (u < u_end) {
-    const int head = it.which / p.row_tiles, tile = it.which - head * p.row_tiles;
-    const int unit_end = u_end - u < it.units - it.unit ? it.unit + static_cast<int>(u_end - u) : it.units;
-    const bool whole = it.unit == 0 && unit_end == it.units;
-    const int tok_begin = it.unit * kUnit;
-    const int tok_end = min(it.tokens, unit_end * kUnit);
-    const int fresh = p.c.new_lens != nullptr ? p.c.new_lens[it.b] : p.seq_len;
+  if (!skip_empty(w)) return;
 
-    // --- loads: a step is two 16-token pieces of keys and of values -------------------------------------
-    const char* side = static_cast<const char*>(p.c.cache) + static_cast<int64_t>(head) * 2 * p.c.page_size * kRow;
-    const int* table = p.c.page_table + it.b * p.c.table_stride;
-    auto load = [&](int tok, int stage) {
+  // The queries of a piece, loaded before the arithmetic of the one before it is finished.
+  uint4 raw[kNT][kG][2];
+  auto load_queries = [&]() {
+    const int head = w.it.which / p.row_tiles, tile = w.it.which - head * p.row_tiles;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int at = tok + 16 * c;
-        if (at < tok_end) {
-          int page = table[at >> p.page_shift];
-          uint32_t bytes = 16;
-          if (page < 0 || page >= p.c.n_pages) {  // zeros in place of a page that does not exist
-            report(p.c.status, AFA_DEV_BAD_PAGE);
-            page = 0;
-            bytes = 0;
-          }
-          const char* src =
-              side + page * p.c.page_stride + static_cast<int64_t>(at & (p.c.page_size - 1)) * kRow + lane * 16;
-          const uint32_t dst = ring + stage * L::kStageBytes + c * 2 * L::kTileBytes + lane * 16;
+    for (int nt = 0; nt < kNT; ++nt) {
+      const int r = tile * L::kRows + nt * 8 + g;
+      const int i = r / p.group, h = head * p.group + (r - i * p.group);
+      const char* src = p.q + w.it.b * p.q_s[0] + i * p.q_s[1] + h * p.q_s[2] + t * 32;
 #pragma unroll
-          for (int kv = 0; kv < 2; ++kv)
+      for (int gr = 0; gr < kG; ++gr)
 #pragma unroll
-            for (int x = 0; x < L::kTileBytes; x += 512)
-              if (x + 512 <= L::kTileBytes || lane * 16 + x < L::kTileBytes)
-                cp_async16(dst + kv * L::kTileBytes + x, src + static_cast<int64_t>(kv) * p.c.page_size * kRow + x,
-                           bytes);
+        for (int x = 0; x < 2; ++x) {
+          raw[nt][gr][x] = make_uint4(0, 0, 0, 0);
+          if (r < p.rows) raw[nt][gr][x] = *reinterpret_cast<const uint4*>(src + gr * 128 + x * 16);
         }
-      }
-      cp_async_commit();
-    };
-    int tok = tok_begin + warp * kStep;
+    }
+  };
+  load_queries();
+
+  // --- loads run ahead of the arithmetic, through the ends of pieces -----------------------------------
+  // A step is 32 tokens of keys and of values, from one page or from two of 16
+  // tokens.  Lane i looks up the pages of the i-th step from the last look-up on.
+  Walk ahead = w;
+  bool more = true;
+  const char* side = nullptr;  // the head of the piece the loads are in, in page 0
+  const bool small_pages = p.c.page_size < kStep;
+  int page[2] = {0, 0}, page_step = 0;
+  auto look_up = [&]() {
+    page_step = 0;
+    const int at = ahead.tok + lane * kUnit;
+    const int* table = p.c.page_table + ahead.it.b * p.c.table_stride;
+    if (at < ahead.tok_end) page[0] = table[at >> p.page_shift];
+    if (small_pages && at + 16 < ahead.tok_end) page[1] = table[(at + 16) >> p.page_shift];
+  };
+  // To the next piece with tokens for this warp, if the loads have reached the end of theirs.
+  auto settle = [&]() {
+    while (more && ahead.tok >= ahead.tok_end) more = ahead.next(p, warp);
+    if (more) {
+      const int head = ahead.it.which / p.row_tiles;
+      side = static_cast<const char*>(p.c.cache) + static_cast<int64_t>(head) * 2 * p.c.page_size * kRow + lane * 16;
+      look_up();
+    }
+  };
+  // `tokens` rows from place `at` of a page: keys to dst, values kSideBytes behind
+  auto copy = [&](auto tokens, int pg, uint32_t at, uint32_t dst) {
+    constexpr int kBytes = decltype(tokens)::value * kRow;
+    uint32_t bytes = 16;
+    if (static_cast<uint32_t>(pg) >= static_cast<uint32_t>(p.c.n_pages)) {
+      report(p.c.status, AFA_DEV_BAD_PAGE);  // zeros in place of a page that does not exist
+      pg = 0;
+      bytes = 0;
+    }
+    const char* keys = far(far(side, pg, p.page_stride), at, kRow);
+    const char* values = far(keys, p.c.page_size, kRow);
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) load(tok + s * kUnit, s);
+    for (int x = 0; x < kBytes; x += 512)
+      if (x + 512 <= kBytes || lane * 16 + x < kBytes) {
+        cp_async16(dst + x, keys + x, bytes);
+        cp_async16(dst + L::kSideBytes + x, values + x, bytes);
+      }
+  };
+  auto load = [&](uint32_t dst) {  // dst: the stage, and this lane's 16 bytes of it
+    if (more) {
+      const int pg = __shfl_sync(0xffffffffu, page[0], page_step);
+      if (!small_pages) {
+        copy(std::integral_constant<int, kStep>{}, pg, ahead.tok & (p.c.page_size - 1), dst);
+      } else {
+        const int pg1 = __shfl_sync(0xffffffffu, page[1], page_step);
+        copy(std::integral_constant<int, 16>{}, pg, 0, dst);
+        if (ahead.tok + 16 < ahead.tok_end) copy(std::integral_constant<int, 16>{}, pg1, 0, dst + 16 * kRow);
+      }
+      ahead.tok += kUnit;
+      if (ahead.tok >= ahead.tok_end)
+        settle();
+      else if (++page_step == 32)
+        look_up();
+    }
+    cp_async_commit();
+  };
+  settle();
+#pragma unroll 1
+  for (int s = 0; s < kStages - 1; ++s) load(ring + s * L::kStageBytes + lane * 16);
+  int stage = 0;  // of the next step; the one before it is free
+
+  for (;;) {
+    const Item it = w.it;
+    const int head = it.which / p.row_tiles, tile = it.which - head * p.row_tiles;
+    const bool starts = it.unit <= kItemUnits, whole = starts && w.unit_end == it.units;
+    const int fresh = p.c.new_lens != nullptr ? p.c.new_lens[it.b] : p.seq_len;
 
     // --- queries: rows on the N side, their channels in the order the codes come ------------------------
     uint32_t qf[kNT][kG][8];
@@ -270,28 +393,16 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
     int limit_min = it.tokens;
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
-      const int r = tile * L::kRows + nt * 8 + g;
-      const int i = r / p.group, h = head * p.group + (r - i * p.group);
-      uint4 raw[kG][2];
-#pragma unroll
-      for (int gr = 0; gr < kG; ++gr)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          raw[gr][x] = make_uint4(0, 0, 0, 0);
-          if (r < p.rows)
-            raw[gr][x] = *reinterpret_cast<const uint4*>(p.q + it.b * p.q_s[0] + i * p.q_s[1] + h * p.q_s[2] +
-                                                         gr * 128 + t * 32 + x * 16);
-        }
       float big = 0.0f, sum[kG];
 #pragma unroll
       for (int gr = 0; gr < kG; ++gr) {
         sum[gr] = 0.0f;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const uint32_t w[4] = {raw[gr][x].x, raw[gr][x].y, raw[gr][x].z, raw[gr][x].w};
+          const uint32_t v4[4] = {raw[nt][gr][x].x, raw[nt][gr][x].y, raw[nt][gr][x].z, raw[nt][gr][x].w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 v = unpack2<kBF16>(w[e]);
+            const float2 v = unpack2<kBF16>(v4[e]);
             big = fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y)));
             sum[gr] += v.x + v.y;
           }
@@ -312,11 +423,11 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
       for (int gr = 0; gr < kG; ++gr)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const uint32_t w[4] = {raw[gr][x].x, raw[gr][x].y, raw[gr][x].z, raw[gr][x].w};
+          const uint32_t v4[4] = {raw[nt][gr][x].x, raw[nt][gr][x].y, raw[nt][gr][x].z, raw[nt][gr][x].w};
           float v[8];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            const float2 f = unpack2<kBF16>(w[y]);
+            const float2 f = unpack2<kBF16>(v4[y]);
             v[2 * y] = f.x * up;
             v[2 * y + 1] = f.y * up;
           }
@@ -340,14 +451,17 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
     if (p.causal) limit_min = min(it.tokens, max(0, it.tokens - fresh + tile * L::kRows / p.group + 1));
 
     // --- the walk over the tokens ------------------------------------------------------------------------
-    float m_ref[kNT][2], l[kNT][2], e_ref[kG], inv_e[kG];
+    // A weight is held as p = 2^(score + off): off takes off the row's reference maximum (none yet: -inf) and the
+    // power of two above the largest step so far, so that p s' stays within 2^(kRescale + kHeadroom).
+    float m_ref[kNT][2], off[kNT][2], limit_s[kNT][2], l[kNT][2];
+    float e_max = 0.0f;
     float acc[kNT][kG][4][4], acc_m[kNT][kG][2];
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        m_ref[nt][x] = -INFINITY;
-        l[nt][x] = 0.0f;
+        m_ref[nt][x] = limit_s[nt][x] = -INFINITY;
+        off[nt][x] = l[nt][x] = 0.0f;
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
           acc_m[nt][gr][x] = 0.0f;
@@ -355,70 +469,65 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
           for (int mt = 0; mt < 4; ++mt) acc[nt][gr][mt][x] = acc[nt][gr][mt][2 + x] = 0.0f;
         }
       }
-#pragma unroll
-    for (int gr = 0; gr < kG; ++gr) {
-      e_ref[gr] = 0.0f;
-      inv_e[gr] = 0.0f;
-    }
 
-    auto compute = [&](auto masked_tag, int tok0, uint32_t base) {
+    // Values' codes are multiplied with a mean taken off, which m' gives back: the accumulators then stay near the
+    // result instead of growing with the 7.5 s' a token that m' would take off at the end -- their roundings with
+    // them, which the matrix instruction makes towards zero.  For an fp16 result 8 from every code, by an exact
+    // fp16 subtraction (relative error 2.9e-4 against 5.5e-4 without; the output's own rounding is 2.1e-4).  For
+    // bf16 (1.7e-3) 15 from odd tokens only, which costs nothing and leaves the sum's mean near zero as well.
+    const float taken = g & 1 ? 15.0f : 0.0f;
+
+    // 16 tokens from tok0 on, at `kb` (keys) and behind them (values)
+    auto compute = [&](auto masked_tag, int tok0, const char* kb) {
       constexpr bool kMasked = decltype(masked_tag)::value;
-      float s[2][kNT][4];
-      float vs[2][2][kG], vm[2][2][kG];  // s' and m' of tokens g, g + 8 of each 16
-      float vs_max[kG];
-#pragma unroll
-      for (int gr = 0; gr < kG; ++gr) vs_max[gr] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t kb = base + c * 2 * L::kTileBytes;
-        float part[kNT][4], mins[kNT][4];
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) part[nt][x] = mins[nt][x] = 0.0f;
+      float s[kNT][4];
+      float vs[2][kG], vm[2][kG];  // s' and what m' becomes (below) of tokens g, g + 8
+      float vs_max = 0.0f;
+      {
         uint32_t par[2][2][kG];  // keys, values; tokens g, g + 8
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const uint32_t a = kb + kv * L::kTileBytes + (g + 8 * y) * kRow + kD / 2;
+            const char* a = kb + kv * L::kSideBytes + (g + 8 * y) * kRow + kD / 2;
             if constexpr (kG == 2) {
-              const uint2 w = lds64(a);
-              par[kv][y][0] = w.x;
-              par[kv][y][1] = w.y;
+              const uint2 v = lds64(a);
+              par[kv][y][0] = v.x;
+              par[kv][y][1] = v.y;
             } else {
               par[kv][y][0] = lds32(a);
             }
           }
+        float part[kNT][4], mins[kNT][4];
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
-          uint32_t w[2][2];
+          uint32_t v[2][2];
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const uint32_t a = kb + (g + 8 * y) * kRow + gr * 32 + t * 8;
+            const char* a = kb + (g + 8 * y) * kRow + gr * 32 + t * 8;
             if constexpr (kG == 2) {
-              const uint2 v = lds64(a);
-              w[y][0] = v.x;
-              w[y][1] = v.y;
+              const uint2 x = lds64(a);
+              v[y][0] = x.x;
+              v[y][1] = x.y;
             } else {  // rows of 36 bytes: 4-byte loads
-              w[y][0] = lds32(a);
-              w[y][1] = lds32(a + 4);
+              v[y][0] = lds32(a);
+              v[y][1] = lds32(a + 4);
             }
           }
           float dot[kNT][4];
 #pragma unroll
-          for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) dot[nt][x] = 0.0f;
-#pragma unroll
           for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
-              const uint32_t lo = w[0][x] >> (8 * z), hi = w[1][x] >> (8 * z);
+              const uint32_t lo = v[0][x] >> (8 * z), hi = v[1][x] >> (8 * z);
 #pragma unroll
-              for (int nt = 0; nt < kNT; ++nt)
-                mma16816(dot[nt], lo & 0x000f000fu, hi & 0x000f000fu, lo & 0x00f000f0u, hi & 0x00f000f0u,
-                         qf[nt][gr][x * 4 + z * 2], qf[nt][gr][x * 4 + z * 2 + 1]);
+              for (int nt = 0; nt < kNT; ++nt) {
+                const uint32_t b0 = qf[nt][gr][x * 4 + z * 2], b1 = qf[nt][gr][x * 4 + z * 2 + 1];
+                if (x == 0 && z == 0)
+                  mma16816_new(dot[nt], lo & 0x000f000fu, hi & 0x000f000fu, lo & 0x00f000f0u, hi & 0x00f000f0u, b0, b1);
+                else
+                  mma16816(dot[nt], lo & 0x000f000fu, hi & 0x000f000fu, lo & 0x00f000f0u, hi & 0x00f000f0u, b0, b1);
+              }
             }
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
@@ -427,153 +536,164 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
             for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
-                part[nt][2 * y + x] = fmaf(sm.x, dot[nt][2 * y + x], part[nt][2 * y + x]);
-                mins[nt][2 * y + x] = fmaf(sm.y, qs[nt][gr][x], mins[nt][2 * y + x]);
+                part[nt][2 * y + x] = gr == 0 ? sm.x * dot[nt][2 * y + x] : fmaf(sm.x, dot[nt][2 * y + x], part[nt][2 * y + x]);
+                mins[nt][2 * y + x] = fmaf(sm.y, qs[nt][gr][x], gr == 0 ? off[nt][x] : mins[nt][2 * y + x]);
               }
           }
         }
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          const int at = tok0 + 16 * c + g + 8 * y;
+          const int at = tok0 + g + 8 * y;
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               float v = fmaf(a_of[nt][x], part[nt][2 * y + x], mins[nt][2 * y + x]);
               if (kMasked && at >= limit[nt][x]) v = -INFINITY;
-              s[c][nt][2 * y + x] = v;
+              s[nt][2 * y + x] = v;
             }
 #pragma unroll
           for (int gr = 0; gr < kG; ++gr) {
             float2 sm = unpack2<kBF16>(par[1][y][gr]);
             if (kMasked && at >= it.tokens) sm = make_float2(0.0f, 0.0f);  // not a token: whatever the page held
-            vs[c][y][gr] = sm.x;
-            vm[c][y][gr] = sm.y;
-            vs_max[gr] = fmaxf(vs_max[gr], fabsf(sm.x));
+            vs[y][gr] = sm.x;
+            vm[y][gr] = fmaf(kBF16 ? taken : 8.0f, sm.x, sm.y);
+            vs_max = fmaxf(vs_max, fabsf(sm.x));
           }
         }
       }
 
-      // New references only where a score passes the old one by 2^kRescale, or a step the old scale.
-      bool moved = false;
+      // New references only where a score passes the old one by 2^kRescale, or a step the old power of two.
+      bool moved = vs_max > e_max;
       float top[kNT][2];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          top[nt][x] = fmaxf(fmaxf(s[0][nt][x], s[0][nt][2 + x]), fmaxf(s[1][nt][x], s[1][nt][2 + x]));
-          moved |= top[nt][x] > m_ref[nt][x] + kRescale;
+          top[nt][x] = fmaxf(s[nt][x], s[nt][2 + x]);
+          moved |= top[nt][x] > limit_s[nt][x];
         }
-#pragma unroll
-      for (int gr = 0; gr < kG; ++gr) moved |= vs_max[gr] > e_ref[gr];
       if (__any_sync(0xffffffffu, moved)) {
-        float by_e[kG];
-#pragma unroll
-        for (int gr = 0; gr < kG; ++gr) {
-          const float big = max_over_rows(vs_max[gr]);
-          by_e[gr] = 1.0f;
-          if (big > e_ref[gr]) {
-            // the power of two above, from 2^-90 on, so that its reciprocal is normal too
-            const uint32_t ex = min(max(__float_as_uint(big) >> 23, 36u), 252u) + 1u;
-            const float now = __uint_as_float(ex << 23);
-            by_e[gr] = e_ref[gr] / now;
-            e_ref[gr] = now;
-            inv_e[gr] = __uint_as_float((254u - ex) << 23) * kPScale;
-          }
+        const float seen = max_over_rows(vs_max);
+        if (seen > e_max) {
+          // the power of two above, from 2^-60 (so that p times a minimum stays far from fp32's largest) to 2^126
+          const uint32_t ex = min(max(__float_as_uint(seen) >> 23, 66u), 252u) + 1u;
+          e_max = __uint_as_float(ex << 23);
         }
+        const float e = e_max > 0.0f ? static_cast<float>(static_cast<int>(__float_as_uint(e_max) >> 23) - 127) : 0.0f;
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const float now = fmaxf(m_ref[nt][x], max_over_rows(top[nt][x]));
-            const float by = now == -INFINITY ? 1.0f : ex2_approx(m_ref[nt][x] - now);
+            const float now = fmaxf(m_ref[nt][x], max_over_rows(top[nt][x] - off[nt][x]));
+            const float to = now == -INFINITY ? 0.0f : kHeadroom - e - now;
+            const float shift = to - off[nt][x];
+            const float by = m_ref[nt][x] == -INFINITY ? 1.0f : ex2_approx(shift);
+            limit_s[nt][x] = now == -INFINITY ? -INFINITY : kRescale + kHeadroom - e;
             m_ref[nt][x] = now;
+            off[nt][x] = to;
+            s[nt][x] += shift;
+            s[nt][2 + x] += shift;
             l[nt][x] *= by;
 #pragma unroll
             for (int gr = 0; gr < kG; ++gr) {
               acc_m[nt][gr][x] *= by;
 #pragma unroll
               for (int mt = 0; mt < 4; ++mt) {
-                acc[nt][gr][mt][x] *= by * by_e[gr];
-                acc[nt][gr][mt][2 + x] *= by * by_e[gr];
+                acc[nt][gr][mt][x] *= by;
+                acc[nt][gr][mt][2 + x] *= by;
               }
             }
           }
       }
 
+      const char* vb = kb + L::kSideBytes;
+      uint32_t pf[kNT][kG][2];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t vb = base + (c * 2 + 1) * L::kTileBytes;
-        uint32_t pf[kNT][kG][2];
+      for (int nt = 0; nt < kNT; ++nt) {
+        float pr[4];
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-          float pr[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float ref = m_ref[nt][x & 1];
-            pr[x] = ex2_approx(s[c][nt][x] - (kMasked && ref == -INFINITY ? 0.0f : ref));
-            l[nt][x & 1] += pr[x];
-          }
-#pragma unroll
-          for (int gr = 0; gr < kG; ++gr)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const float sc = vs[c][y][gr] * inv_e[gr];
-              float w[2];
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const float pp = pr[2 * y + x];
-                w[x] = pp * sc;
-                float mm = vm[c][y][gr];
-                if (kMasked && tok0 + 16 * c + g + 8 * y >= limit[nt][x]) {  // its s' and m' may be NaN
-                  w[x] = 0.0f;
-                  mm = 0.0f;
-                }
-                acc_m[nt][gr][x] = fmaf(pp, mm, acc_m[nt][gr][x]);
-              }
-              pf[nt][gr][y] = transpose8x8(half2_of(w[0], w[1]));
-            }
+        for (int x = 0; x < 4; ++x) {
+          pr[x] = ex2_approx(s[nt][x]);
+          l[nt][x & 1] += pr[x];
         }
 #pragma unroll
-        for (int gr = 0; gr < kG; ++gr) {
-          // rows of tokens 2t, 2t + 1, 2t + 8, 2t + 9; channels 8g .. 8g + 7 of the group
-          const uint32_t a = vb + 2 * t * kRow + gr * 32 + g * 4;
-          const uint32_t w0 = lds32(a), w1 = lds32(a + kRow), w2 = lds32(a + 8 * kRow), w3 = lds32(a + 9 * kRow);
+        for (int gr = 0; gr < kG; ++gr)
 #pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const uint32_t sel = z ? 0x7632u : 0x5410u;
-            const uint32_t lo = __byte_perm(w0, w1, sel), hi = __byte_perm(w2, w3, sel);
+          for (int y = 0; y < 2; ++y) {
+            float ps[2];
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const uint32_t lo8 = lo >> (8 * y), hi8 = hi >> (8 * y);
+            for (int x = 0; x < 2; ++x) {
+              const float pp = pr[2 * y + x];
+              ps[x] = pp * vs[y][gr];
+              float mm = vm[y][gr];
+              if (kMasked && tok0 + g + 8 * y >= limit[nt][x]) {  // its s' and m' may be NaN
+                ps[x] = 0.0f;
+                mm = 0.0f;
+              }
+              acc_m[nt][gr][x] = fmaf(pp, mm, acc_m[nt][gr][x]);
+            }
+            pf[nt][gr][y] = transpose8x8(half2_of(ps[0], ps[1]));
+          }
+      }
 #pragma unroll
-              for (int nt = 0; nt < kNT; ++nt)
-                mma16816(acc[nt][gr][2 * z + y], lo8 & 0x000f000fu, lo8 & 0x00f000f0u, hi8 & 0x000f000fu,
-                         hi8 & 0x00f000f0u, pf[nt][gr][0], pf[nt][gr][1]);
+      for (int gr = 0; gr < kG; ++gr) {
+        // rows of tokens 2t, 2t + 1, 2t + 8, 2t + 9; channels 8g .. 8g + 7 of the group
+        const char* a = vb + 2 * t * kRow + gr * 32 + g * 4;
+        const uint32_t w0 = lds32(a), w1 = lds32(a + kRow), w2 = lds32(a + 8 * kRow), w3 = lds32(a + 9 * kRow);
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const uint32_t sel = z ? 0x7632u : 0x5410u;
+          const uint32_t lo = __byte_perm(w0, w1, sel), hi = __byte_perm(w2, w3, sel);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t lo8 = lo >> (8 * y), hi8 = hi >> (8 * y);
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt) {
+              float(&d)[4] = acc[nt][gr][2 * z + y];
+              const uint32_t b0 = pf[nt][gr][0], b1 = pf[nt][gr][1];
+              if constexpr (kBF16) {
+                // c' and c' - 15 by turns (odd tokens, the high halves)
+                mma16816(d, pick(lo8, 0x000f000fu, 0x800f0000u), pick(lo8, 0x00f000f0u, 0x80f00000u),
+                         pick(hi8, 0x000f000fu, 0x800f0000u), pick(hi8, 0x00f000f0u, 0x80f00000u), b0, b1);
+              } else {
+                // c' - 8, and 16 times that
+                mma16816(d, sub2((lo8 & 0x000f000fu) | 0x64006400u, 0x64086408u),
+                         sub2((lo8 & 0x00f000f0u) | 0x64006400u, 0x64806480u),
+                         sub2((hi8 & 0x000f000fu) | 0x64006400u, 0x64086408u),
+                         sub2((hi8 & 0x00f000f0u) | 0x64006400u, 0x64806480u), b0, b1);
+              }
             }
           }
         }
       }
     };
 
-    int stage = 0;
-    for (; tok < tok_end; tok += kUnit) {
+    for (; w.tok < w.tok_end; w.tok += kUnit) {
       cp_async_wait<kStages - 2>();
       __syncwarp();  // every lane's part of the step has landed, and the stage loaded next has been read
-      const int next = stage == 0 ? kStages - 1 : stage - 1;
-      load(tok + (kStages - 1) * kUnit, next);
-      const uint32_t base = ring + stage * L::kStageBytes;
-      if (tok + kStep <= limit_min)
-        compute(std::false_type{}, tok, base);
-      else
-        compute(std::true_type{}, tok, base);
+      load(ring + (stage == 0 ? kStages - 1 : stage - 1) * L::kStageBytes + lane * 16);
+      const char* base = smem + warp * L::kWarpBytes + stage * L::kStageBytes;
+      if (w.tok + kStep <= limit_min) {
+        compute(std::false_type{}, w.tok, base);
+        compute(std::false_type{}, w.tok + 16, base + 16 * kRow);
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < 2 && w.tok + 16 * c < w.tok_end; ++c)
+          compute(std::true_type{}, w.tok + 16 * c, base + c * 16 * kRow);
+      }
       stage = stage + 1 == kStages ? 0 : stage + 1;
     }
-    cp_async_wait<0>();
     __syncwarp();
 
+    const bool go = w.next(p, warp) && skip_empty(w);
+    if (go) load_queries();
+
     // --- the warps' shares -> the CTA's -------------------------------------------------------------------
-    float* mine = reinterpret_cast<float*>(smem + warp * L::kWarpBytes);  // [row][channel]
+    const uint32_t place = L::kInStage ? warp * L::kWarpBytes + (stage == 0 ? kStages - 1 : stage - 1) * L::kStageBytes
+                                       : kWarps * L::kWarpBytes + warp * L::kShareBytes;
+    float* mine = reinterpret_cast<float*>(smem + place);  // [row][channel]
+    if (lane == 0) places[warp] = place;
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
@@ -581,13 +701,14 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
         const int row = nt * 8 + 2 * t + x;
         const float sum = sum_over_rows(l[nt][x]);
         if (g == 0) {
-          stats[(warp * L::kRows + row) * 2] = m_ref[nt][x];
+          stats[(warp * L::kRows + row) * 2] = m_ref[nt][x] == -INFINITY ? -INFINITY : -off[nt][x];
           stats[(warp * L::kRows + row) * 2 + 1] = sum;
         }
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
           const float mn = sum_over_rows(acc_m[nt][gr][x]);
-          const float even = e_ref[gr] * (16777216.0f / kPScale), odd = e_ref[gr] * (1048576.0f / kPScale);
+          // what the codes' places left out
+          const float even = kBF16 ? 16777216.0f : 1.0f, odd = kBF16 ? 1048576.0f : 0.0625f;
           float* dst = mine + row * kD + gr * 64 + g * 8;
 #pragma unroll
           for (int mt = 0; mt < 4; mt += 2)
@@ -598,26 +719,26 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
       }
     __syncthreads();
     // A range that starts within an item is the CTA's first, one that ends within an item its last.
-    float* share = p.ws + (static_cast<int64_t>(cta) * 2 + (it.unit == 0 ? 1 : 0)) * L::kShare;
+    float* share = p.ws + (static_cast<int64_t>(blockIdx.x) * 2 + (starts ? 1 : 0)) * L::kShare;
     for (int i = threadIdx.x; i < L::kRows * (kD / 4); i += kThreads) {
       const int row = i / (kD / 4), c4 = i - row * (kD / 4);
       float m[kWarps], top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        m[w] = stats[(w * L::kRows + row) * 2];
-        top = fmaxf(top, m[w]);
+      for (int v = 0; v < kWarps; ++v) {
+        m[v] = stats[(v * L::kRows + row) * 2];
+        top = fmaxf(top, m[v]);
       }
       float sum = 0.0f;
       float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float by = m[w] == -INFINITY && top == -INFINITY ? 1.0f : ex2_approx(m[w] - top);
-        sum = fmaf(by, stats[(w * L::kRows + row) * 2 + 1], sum);
-        const float4 v = *reinterpret_cast<const float4*>(smem + w * L::kWarpBytes + (row * kD + c4 * 4) * 4);
-        o.x = fmaf(by, v.x, o.x);
-        o.y = fmaf(by, v.y, o.y);
-        o.z = fmaf(by, v.z, o.z);
-        o.w = fmaf(by, v.w, o.w);
+      for (int v = 0; v < kWarps; ++v) {
+        const float by = m[v] == -INFINITY && top == -INFINITY ? 1.0f : ex2_approx(m[v] - top);
+        sum = fmaf(by, stats[(v * L::kRows + row) * 2 + 1], sum);
+        const float4 f = *reinterpret_cast<const float4*>(smem + places[v] + (row * kD + c4 * 4) * 4);
+        o.x = fmaf(by, f.x, o.x);
+        o.y = fmaf(by, f.y, o.y);
+        o.z = fmaf(by, f.z, o.z);
+        o.w = fmaf(by, f.w, o.w);
       }
       const int r = tile * L::kRows + row;
       if (whole) {
@@ -640,75 +761,73 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
         }
       }
     }
-    __syncthreads();  // the shares have been read: their memory takes the next item's steps
-
-    u += unit_end - it.unit;
-    it.unit = 0;
-    if (++it.which == p.c.n_kv_heads * p.row_tiles && u < u_end) {
-      it.which = 0;
-      ++it.b;
-      it.tokens = tokens_of(p, it.b);
-      it.units = units_of(it.tokens);
-    }
+    __syncthreads();  // the shares have been read: their memory takes the next steps
+    if (!go) break;
   }
+  cp_async_wait<0>();
 }
 
 // Joins the shares of the items that several CTAs worked on: CTA i takes the
 // item its range starts within, if the CTA before it holds that item's start;
 // one warp a row (blockIdx.y).  The shares are added in the order of the CTAs.
+// Launched while the first kernel still runs: it finds its item meanwhile and
+// waits for that kernel's end before it reads a share.
 template <int kD, bool kBF16, int kNT>
 __global__ void __launch_bounds__(128) cache4_join_kernel(const FwdParams4 p) {
   using L = FwdLayout4<kD, kNT>;
   constexpr int kPer = kD / 32;  // channels of a lane
   const int lane = threadIdx.x & 31;
   const int per = (p.c.batch + 31) / 32;
-  long long before_lane;
-  const Division div = divide(p, per, &before_lane);
-  const int cta = blockIdx.x;
-  if (cta == 0 || cta >= div.ctas) return;
-  const long long u = div.first(cta);
-  const Item it = find_item(p, per, before_lane, u);
-  const long long begin = u - it.unit, end = begin + it.units;
-  if (it.unit == 0 || div.first(cta - 1) > begin) return;
-  const int head = it.which / p.row_tiles, tile = it.which - head * p.row_tiles;
-  const int fresh = p.c.new_lens != nullptr ? p.c.new_lens[it.b] : p.seq_len;
-  for (int row = blockIdx.y * 4 + (threadIdx.x >> 5); row < L::kRows; row += gridDim.y * 4) {
-    const int r = tile * L::kRows + row;
-    if (r >= p.rows) break;
-    auto share = [&](int i) { return p.ws + (static_cast<int64_t>(i) * 2 + (i == cta - 1 ? 1 : 0)) * L::kShare; };
-    float top = -INFINITY;
-    int last = cta;
-    while (last + 1 < div.ctas && div.first(last + 1) < end) ++last;
-    for (int i = cta - 1 + lane; i <= last; i += 32) top = fmaxf(top, share(i)[L::kRows * kD + row * 2]);
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    float sum = 0.0f, o[kPer];
-#pragma unroll
-    for (int x = 0; x < kPer; ++x) o[x] = 0.0f;
-#pragma unroll 4
-    for (int i = cta - 1; i <= last; ++i) {
-      const float* sh = share(i);
-      const float m = sh[L::kRows * kD + row * 2];
-      const float by = m == -INFINITY && top == -INFINITY ? 1.0f : ex2_approx(m - top);
-      sum = fmaf(by, sh[L::kRows * kD + row * 2 + 1], sum);
-#pragma unroll
-      for (int x = 0; x < kPer; x += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(sh + row * kD + lane * kPer + x);
-        o[x] = fmaf(by, v.x, o[x]);
-        o[x + 1] = fmaf(by, v.y, o[x + 1]);
-      }
-    }
-    const int n = r / p.group, h = head * p.group + (r - n * p.group);
-    const bool some = n < fresh && !(sum == 0.0f);
-    const float inv = some ? 1.0f / sum : 0.0f;
-    char* dst = p.o + it.b * p.o_s[0] + n * p.o_s[1] + h * p.o_s[2] + lane * kPer * 2;
-#pragma unroll
-    for (int x = 0; x < kPer; x += 2)
-      *reinterpret_cast<uint32_t*>(dst + x * 2) = some ? pack2<kBF16>(o[x] * inv, o[x + 1] * inv) : 0u;
-    if (p.lse != nullptr && lane == 0)
-      p.lse[(static_cast<int64_t>(it.b) * p.n_heads + h) * p.seq_len + n] =
-          some ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+  int before_lane;
+  const Division div = divide(p, per, gridDim.x + 1, &before_lane);
+  const int cta = blockIdx.x + 1;
+  bool mine = cta < div.ctas;
+  int head = 0, tile = 0, fresh = 0, last = 0, b = 0;
+  if (mine) {
+    const int u = div.first(cta);
+    const Item it = find_item(p, per, before_lane, u);
+    const int begin = u - it.unit + kItemUnits, end = u - it.unit + it.units;  // of the tokens' units
+    mine = u > begin && div.first(cta - 1) <= begin;
+    head = it.which / p.row_tiles;
+    tile = it.which - head * p.row_tiles;
+    b = it.b;
+    fresh = p.c.new_lens != nullptr ? p.c.new_lens[b] : p.seq_len;
+    last = div.holder(end - 1);
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!mine) return;
+  const int row = blockIdx.y * 4 + (threadIdx.x >> 5), r = tile * L::kRows + row;
+  if (r >= p.rows) return;
+  auto share = [&](int i) { return p.ws + (static_cast<int64_t>(i) * 2 + (i == cta - 1 ? 1 : 0)) * L::kShare; };
+  // in one pass, so that no load waits for the maximum
+  float top = -INFINITY, sum = 0.0f, o[kPer];
+#pragma unroll
+  for (int x = 0; x < kPer; ++x) o[x] = 0.0f;
+#pragma unroll 8
+  for (int i = cta - 1; i <= last; ++i) {
+    const float* sh = share(i);
+    const float2 ml = *reinterpret_cast<const float2*>(sh + L::kRows * kD + row * 2);
+    const float now = fmaxf(top, ml.x);
+    const float old = now == -INFINITY ? 1.0f : ex2_approx(top - now), by = now == -INFINITY ? 1.0f : ex2_approx(ml.x - now);
+    top = now;
+    sum = fmaf(by, ml.y, sum * old);
+#pragma unroll
+    for (int x = 0; x < kPer; x += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(sh + row * kD + lane * kPer + x);
+      o[x] = fmaf(by, v.x, o[x] * old);
+      o[x + 1] = fmaf(by, v.y, o[x + 1] * old);
+    }
+  }
+  const int n = r / p.group, h = head * p.group + (r - n * p.group);
+  const bool some = n < fresh && !(sum == 0.0f);
+  const float inv = some ? 1.0f / sum : 0.0f;
+  char* dst = p.o + b * p.o_s[0] + n * p.o_s[1] + h * p.o_s[2] + lane * kPer * 2;
+#pragma unroll
+  for (int x = 0; x < kPer; x += 2)
+    *reinterpret_cast<uint32_t*>(dst + x * 2) = some ? pack2<kBF16>(o[x] * inv, o[x + 1] * inv) : 0u;
+  if (p.lse != nullptr && lane == 0)
+    p.lse[(static_cast<int64_t>(b) * p.n_heads + h) * p.seq_len + n] =
+        some ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -736,8 +855,16 @@ cudaError_t launch4(const FwdParams4& p, unsigned grid, cudaStream_t s) {
   cache4_fwd_kernel<kD, kBF16, kNT><<<grid, kThreads, L::kSmem, s>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || grid == 1) return e;
-  cache4_join_kernel<kD, kBF16, kNT><<<dim3(grid, L::kRows / 4), 128, 0, s>>>(p);
-  return cudaGetLastError();
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid - 1, L::kRows / 4);
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cfg.attrs = &overlap;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, cache4_join_kernel<kD, kBF16, kNT>, p);
 }
 
 #define AFA_KERNEL4(D, BF, NT)                                                                                 \
@@ -764,10 +891,11 @@ int plan4(const AfaCache4* c, int32_t seq_len, int32_t n_heads, const Kernel4** 
   const int di = c->head_dim == 128, ti = c->dtype == AFA_DTYPE_BF16, ni = rows > 8;
   const Kernel4& k = kKernels4[di][ti][ni];
   const int64_t tiles = (rows + k.rows - 1) / k.rows;
-  // items and units are counted in 32 and 64 bits, with a factor of the grid's size to spare
+  if (c->n_pages > 1 && c->page_stride > UINT32_MAX) return AFA_ERR_TOO_LARGE;
+  // units are counted in 31 bits
   const int64_t items = tiles * c->n_kv_heads;
-  const int64_t units = (int64_t{c->max_pages} * c->page_size + kUnit - 1) / kUnit;
-  if (items > INT32_MAX || items * c->batch > (int64_t{1} << 48) / units) return AFA_ERR_TOO_LARGE;
+  const int64_t units = (int64_t{c->max_pages} * c->page_size + kUnit - 1) / kUnit + kItemUnits;
+  if (items > INT32_MAX || items * c->batch > INT32_MAX / units) return AFA_ERR_TOO_LARGE;
   int dev = 0, sms = 0;
   rc = ops_device(&dev, &sms);
   if (rc != AFA_OK) return rc;
@@ -838,8 +966,8 @@ int afa_cache4_fwd_sm100(const AfaCache4* cache, const AfaCache4FwdArgs* a, void
   p.rows = a->seq_len * p.group;
   p.row_tiles = tiles;
   p.page_shift = ops_log2(cache->page_size);
+  p.page_stride = static_cast<uint32_t>(cache->page_stride);
   p.causal = a->causal;
-  p.min_units = 1;
   const double scale = a->scale > 0.f ? a->scale : 1.0 / (cache->head_dim == 64 ? 8.0 : 11.313708498984761);
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   if (k->launch(p, static_cast<unsigned>(grid), static_cast<cudaStream_t>(stream)) != cudaSuccess) {

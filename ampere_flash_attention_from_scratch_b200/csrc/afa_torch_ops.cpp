@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -33,12 +34,19 @@ using afa_torch::status_word;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// The compute capability of a device never changes: looked up once for each.
 void check_arch(int dev) {
-  int major = 0, minor = 0;
-  cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-  cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
-  TORCH_CHECK(major == 10 && minor == 0, "Flash Attention (sm_100a build) requires SM_100 (current: SM_", major, ".",
-              minor, ")");
+  static std::atomic<int> known[64];  // 10 * major + minor, 0: not looked up
+  const bool kept = dev >= 0 && dev < 64;
+  int cc = kept ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (cc == 0) {
+    int major = 0, minor = 0;
+    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+    cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
+    cc = 10 * major + minor;
+    if (kept) known[dev].store(cc, std::memory_order_relaxed);
+  }
+  TORCH_CHECK(cc == 100, "Flash Attention (sm_100a build) requires SM_100 (current: SM_", cc / 10, ".", cc % 10, ")");
 }
 
 void check_positive(const at::Tensor& t, const char* name) {

@@ -131,7 +131,7 @@ inline int ops_check_cache(const AfaCache4* c) {
   const int64_t page_bytes = int64_t{2} * c->n_kv_heads * c->page_size * afa_cache4_row_bytes(c->head_dim);
   if (c->n_pages > 1 && c->page_stride < page_bytes) return AFA_ERR_INVALID_ARGUMENT;
   if (c->batch > 1 && c->table_stride < 0) return AFA_ERR_INVALID_ARGUMENT;
-  if (int64_t{1} * c->max_pages * c->page_size > INT32_MAX - 512) return AFA_ERR_TOO_LARGE;
+  if (int64_t{1} * c->max_pages * c->page_size > INT32_MAX - 8192) return AFA_ERR_TOO_LARGE;
   return AFA_OK;
 }
 
