@@ -8,9 +8,9 @@
 // are those of the exact quotients (below), so a row's bytes do not depend on
 // how the arithmetic is arranged.
 //
-// Bound: HBM.  A value costs 2 bytes on one side and 0.5625 on the other.  Eight
-// neighbouring lanes hold one group, eight channels (16 bytes) a lane; minimum
-// and maximum travel together as one packed pair through three shuffles.  A CTA
+// Bound: HBM.  A value costs 2 bytes on one side and 0.5625 on the other.  Four
+// neighbouring lanes hold one group, sixteen channels (32 bytes, one access) a lane;
+// minimum and maximum travel together as one packed pair through two shuffles.  A CTA
 // takes a tile of tokens of one sequence times (head, keys or values), tokens
 // fastest, so that the rows it writes are neighbours in a page.
 #include "ops_common.cuh"
@@ -20,7 +20,7 @@ namespace {
 using namespace afa100;
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // rows a lane has in flight
+constexpr int kUnroll = 2;  // rows a lane has in flight
 
 struct Cache4Params {
   AfaCache4 c;
@@ -95,110 +95,188 @@ __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
   return r;
 }
 
-// Eight channels of one lane to eight codes; the lane's group is the eight lanes
-// that differ in the lowest three bits.  *params: s and m.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return r;
+}
+
+// Two quotients of each of eight values, 2^-20 below and above the exact one (the
+// difference, the reciprocal and the product are off by less than 2^-21 together),
+// each rounded to an integer by the addition of 1.5 * 2^23 in the same operation.
+// Where both round alike, so does the exact one; a tie or nearly one (common among
+// values of 8 bits) shows as two neighbours, and the exact difference decides.
 template <bool kBF16>
-__device__ __forceinline__ uint32_t quantise8(const uint4 x, uint32_t* params) {
-  uint32_t lo = min2_nan<kBF16>(min2_nan<kBF16>(x.x, x.y), min2_nan<kBF16>(x.z, x.w));
-  uint32_t hi = max2_nan<kBF16>(max2_nan<kBF16>(x.x, x.y), max2_nan<kBF16>(x.z, x.w));
-  // {minimum, -maximum}, so that one minimum a shuffle carries both
-  uint32_t mm = min2_nan<kBF16>(__byte_perm(lo, hi ^ 0x80008000u, 0x5410), __byte_perm(lo, hi ^ 0x80008000u, 0x7632));
-#pragma unroll
-  for (int i = 1; i < 8; i <<= 1) mm = min2_nan<kBF16>(mm, __shfl_xor_sync(0xffffffffu, mm, i));
-  const float2 ends = unpack2<kBF16>(mm);
-  const float low = ends.x, high = -ends.y;
-  if (!(high - low < __int_as_float(0x7f800000))) {  // an infinity, a NaN, or a range beyond fp32
-    *params = 0x7fff7fffu;
-    return 0u;
-  }
-  const uint32_t s16 = step16<kBF16>(high, low);
-  *params = s16 | (mm << 16);
-  const float s = unpack2<kBF16>(s16).x;
-  if (s == 0.0f) return 0u;
-  // The quick quotient is within 2^-18 of the exact one (15 * 2^-22): unless it is
-  // that close to halfway, it rounds the same.
-  const float inv = 1.0f / s;
-  bool close = s < 1e-30f;
-  uint32_t word = 0;
-  const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+__device__ __forceinline__ uint32_t codes8(const uint32_t (&xs)[4], float low, float s, float below, float above) {
+  const float2 big = make_float2(12582912.0f, 12582912.0f);
+  uint32_t a[8], differ = 0, word = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 v = unpack2<kBF16>(xs[i]);
-    const float q0 = fminf((v.x - low) * inv, 15.0f), q1 = fminf((v.y - low) * inv, 15.0f);
-    const float r0 = rintf(q0), r1 = rintf(q1);
-    close |= fmaxf(fabsf(q0 - r0), fabsf(q1 - r1)) > 0.5f - 7.62939453125e-06f;
-    word |= static_cast<uint32_t>(__float2int_rn(fmaf(r1, 16.0f, r0))) << (8 * i);
+    const float2 v = add2(unpack2<kBF16>(xs[i]), make_float2(-low, -low));
+    const float2 r = fma2(v, make_float2(below, below), big), t = fma2(v, make_float2(above, above), big);
+    a[2 * i] = __float_as_uint(r.x);
+    a[2 * i + 1] = __float_as_uint(r.y);
+    differ |= (__float_as_uint(r.x) ^ __float_as_uint(t.x)) | (__float_as_uint(r.y) ^ __float_as_uint(t.y));
   }
-  if (close) {
-    word = 0;
-#pragma unroll 1
+  // the integers' bits are 0x4b400000 + code: their sum over 16^i carries a constant with it
+#pragma unroll
+  for (int i = 7; i >= 0; --i) word = word * 16u + a[i];
+  word -= 0x4b400000u * 0x11111111u;
+  if (differ != 0) {
+    const float half = 0.5f * s;
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t w = i < 4 ? (i < 2 ? x.x : x.y) : (i < 6 ? x.z : x.w);
-      const float2 v = unpack2<kBF16>(w);
-      word |= code_exact(i & 1 ? v.y : v.x, low, s) << (4 * i);
+      const float2 v2 = unpack2<kBF16>(xs[i / 2]);
+      const float v = i & 1 ? v2.y : v2.x;
+      if (__float_as_uint(fmaf(v - low, above, 12582912.0f)) != a[i]) {
+        const uint32_t c = a[i] & 15u;
+        const float border = fmaf(static_cast<float>(c), s, half), d = sub_odd(v, low);
+        if (d > border || (d == border && (c & 1u))) word += 1u << (4 * i);
+      }
     }
   }
   return word;
 }
 
-// Where the CTA's row `r` is: its token, its side (head * 2 + keys or values) and
-// whether it exists.
-struct RowAt {
-  int token;
-  int side;
-};
+// Sixteen channels of one lane to sixteen codes; the lane's group is the four
+// lanes that differ in the lowest two bits.  *params: s and m.
+template <bool kBF16>
+__device__ __forceinline__ uint2 quantise16(const uint32_t (&x)[2][4], uint32_t* params) {
+  uint32_t lo = x[0][0], hi = x[0][0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    lo = min2_nan<kBF16>(lo, x[i / 4][i % 4]);
+    hi = max2_nan<kBF16>(hi, x[i / 4][i % 4]);
+  }
+  hi ^= 0x80008000u;
+  // {minimum, -maximum}, so that one minimum a shuffle carries both
+  uint32_t mm = min2_nan<kBF16>(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+#pragma unroll
+  for (int i = 1; i < 4; i <<= 1) mm = min2_nan<kBF16>(mm, __shfl_xor_sync(0xffffffffu, mm, i));
+  const float2 ends = unpack2<kBF16>(mm);
+  const float low = ends.x, high = -ends.y;
+  if (!(high - low < __int_as_float(0x7f800000))) {  // an infinity, a NaN, or a range beyond fp32
+    *params = 0x7fff7fffu;
+    return make_uint2(0, 0);
+  }
+  const uint32_t s16 = step16<kBF16>(high, low);
+  *params = s16 | (mm << 16);
+  const float s = unpack2<kBF16>(s16).x;
+  if (s == 0.0f) return make_uint2(0, 0);
+  // Steps so small that 16 bits round them by more than 1/30 (fp16), or that their reciprocal is not an fp32
+  // number: the codes one by one.
+  if (s < (kBF16 ? 1e-30f : 1.9073486328125e-06f)) {
+    uint2 word = make_uint2(0, 0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float2 v = unpack2<kBF16>(x[i / 8][i / 2 % 4]);
+      const uint32_t c = code_exact(i & 1 ? v.y : v.x, low, s) << (4 * (i & 7));
+      if (i < 8)
+        word.x |= c;
+      else
+        word.y |= c;
+    }
+    return word;
+  }
+  float inv;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  const float below = inv * 0.99999904632568359375f, above = inv * 1.00000095367431640625f;
+  return make_uint2(codes8<kBF16>(x[0], low, s, below, above), codes8<kBF16>(x[1], low, s, below, above));
+}
 
 template <int kD>
 struct Tile {
-  static constexpr int kLanes = kD / 8;                  // lanes of a row
-  static constexpr int kRows = kThreads / kLanes;        // rows of a CTA at a time
-  static constexpr int kTile = kRows * kUnroll;          // rows of a CTA
-  static constexpr int kRow = kD / 2 + kD / 16;          // bytes of a cache row
+  static constexpr int kLanes = kD / 16;           // lanes of a row, 16 channels each
+  static constexpr int kRows = kThreads / kLanes;  // rows of a CTA at a time
+  static constexpr int kTile = kRows * kUnroll;    // rows of a CTA
+  static constexpr int kRow = kD / 2 + kD / 16;    // bytes of a cache row
 };
 
-// Byte offset of a cache row, or -1 (reported) where its page does not exist.
-template <int kD>
-__device__ __forceinline__ int64_t cache_row(const Cache4Params& p, int b, int pos, int side) {
-  const int page = p.c.page_table[b * p.c.table_stride + (pos >> p.page_shift)];
-  if (page < 0 || page >= p.c.n_pages) {
-    report(p.c.status, AFA_DEV_BAD_PAGE);
-    return -1;
+// A CTA's tile: kTile rows, 2^tile_shift tokens of some sides (head * 2 + keys or
+// values) of one sequence.  Where a sequence's rows fill it (kLong) there is one
+// side, and a thread's rows lie a fixed distance apart.
+template <int kD, bool kLong>
+struct Place {
+  int b, token0, side0;
+  __device__ __forceinline__ explicit Place(const Cache4Params& p) {
+    const int per = p.n_tiles * p.n_sides;
+    b = blockIdx.x / per;
+    const int rest = blockIdx.x - b * per, tile = rest / p.n_sides;
+    token0 = tile << p.tile_shift;
+    side0 = (rest - tile * p.n_sides) * (Tile<kD>::kTile >> p.tile_shift);
   }
-  const int place = pos & (p.c.page_size - 1);
-  return page * p.c.page_stride + (static_cast<int64_t>(side) * p.c.page_size + place) * Tile<kD>::kRow;
+  // Token and side of the thread's u-th row.
+  __device__ __forceinline__ int token(const Cache4Params& p, int u) const {
+    const int r = u * Tile<kD>::kRows + threadIdx.x / Tile<kD>::kLanes;
+    return token0 + (kLong ? r : r & ((1 << p.tile_shift) - 1));
+  }
+  __device__ __forceinline__ int side(const Cache4Params& p, int u) const {
+    const int r = u * Tile<kD>::kRows + threadIdx.x / Tile<kD>::kLanes;
+    return kLong ? side0 : side0 + (r >> p.tile_shift);
+  }
+};
+
+// The lane's 32 bytes of a row of k or v.
+template <int kD>
+__device__ __forceinline__ char* outer_row(const Cache4Params& p, int b, int token, int side) {
+  const int w = side & 1;
+  return p.x[w] + b * p.x_s[w][0] + (side >> 1) * p.x_s[w][2] + token * p.x_s[w][1] +
+         threadIdx.x % Tile<kD>::kLanes * 32;
 }
 
-template <int kD, bool kBF16>
+// The cache's row, or null (reported) where its page does not exist.
+template <int kD>
+__device__ __forceinline__ char* cache_row(const Cache4Params& p, int b, int pos, int side) {
+  const int page = p.c.page_table[b * p.c.table_stride + (pos >> p.page_shift)];
+  if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(p.c.n_pages)) {
+    report(p.c.status, AFA_DEV_BAD_PAGE);
+    return nullptr;
+  }
+  const int64_t of_side = static_cast<int64_t>(side) * p.c.page_size * Tile<kD>::kRow;
+  return static_cast<char*>(p.c.cache) + of_side + page * p.c.page_stride + (pos & (p.c.page_size - 1)) * Tile<kD>::kRow;
+}
+
+template <int kD, bool kBF16, bool kLong>
 __global__ void __launch_bounds__(kThreads) cache4_write_kernel(const Cache4Params p) {
   using T = Tile<kD>;
-  const int b = blockIdx.x / (p.n_tiles * p.n_sides);
-  const int rest = blockIdx.x - b * (p.n_tiles * p.n_sides);
-  const int token0 = (rest / p.n_sides) << p.tile_shift;
-  const int side0 = (rest % p.n_sides) * (T::kTile >> p.tile_shift);
-  const NewRows fresh = new_rows(p.c, b, p.seq_len);
+  const Place<kD, kLong> at(p);
+  const NewRows fresh = new_rows(p.c, at.b, p.seq_len);
+  if (at.token0 >= fresh.count) return;
   const int lane = threadIdx.x % T::kLanes;
-  uint4 x[kUnroll];
-  int64_t at[kUnroll];
+  uint32_t x[kUnroll][2][4];
+  char* row[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int r = u * T::kRows + threadIdx.x / T::kLanes;
-    const int token = token0 + (r & ((1 << p.tile_shift) - 1)), side = side0 + (r >> p.tile_shift);
-    at[u] = -1;
-    x[u] = make_uint4(0, 0, 0, 0);
-    if (token < fresh.count && side < 2 * p.c.n_kv_heads) {
-      at[u] = cache_row<kD>(p, b, fresh.first + token, side);
-      const int w = side & 1;
-      x[u] = ldg_stream(p.x[w] + b * p.x_s[w][0] + token * p.x_s[w][1] + (side >> 1) * p.x_s[w][2] + lane * 16);
+    const int token = at.token(p, u), side = at.side(p, u);
+    row[u] = nullptr;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[u][i / 4][i % 4] = 0;
+    if (token < fresh.count && (kLong || side < 2 * p.c.n_kv_heads)) {
+      load32(x[u], outer_row<kD>(p, at.b, token, side));
+      row[u] = cache_row<kD>(p, at.b, fresh.first + token, side);
     }
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     uint32_t params;
-    const uint32_t word = quantise8<kBF16>(x[u], &params);
-    if (at[u] >= 0) {
-      char* row = static_cast<char*>(p.c.cache) + at[u];
-      *reinterpret_cast<uint32_t*>(row + lane * 4) = word;
-      if (lane % 8 == 0) *reinterpret_cast<uint32_t*>(row + kD / 2 + lane / 8 * 4) = params;
+    const uint2 word = quantise16<kBF16>(x[u], &params);
+    if (row[u] != nullptr) {
+      if constexpr (kD == 128) {
+        *reinterpret_cast<uint2*>(row[u] + lane * 8) = word;
+      } else {  // rows of 36 bytes
+        *reinterpret_cast<uint32_t*>(row[u] + lane * 8) = word.x;
+        *reinterpret_cast<uint32_t*>(row[u] + lane * 8 + 4) = word.y;
+      }
+      if (lane % 4 == 0) *reinterpret_cast<uint32_t*>(row[u] + kD / 2 + lane) = params;
     }
   }
 }
@@ -207,8 +285,7 @@ __global__ void __launch_bounds__(kThreads) cache4_write_kernel(const Cache4Para
 // exact operands).  A 16-bit value with the bits of 1024 (bf16: 128) and the code in its last places is
 // 1024 + c; the subtraction is exact.
 template <bool kBF16>
-__device__ __forceinline__ uint4 dequantise8(uint32_t word, uint32_t params) {
-  const uint32_t s2 = __byte_perm(params, 0, 0x1010), m2 = __byte_perm(params, 0, 0x3232);
+__device__ __forceinline__ void dequantise8(uint32_t (&out)[4], uint32_t word, uint32_t s2, uint32_t m2) {
   uint32_t v[4];  // channels {0, 4}, {1, 5}, {2, 6}, {3, 7}
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -225,42 +302,47 @@ __device__ __forceinline__ uint4 dequantise8(uint32_t word, uint32_t params) {
       asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v[i]) : "r"(f), "r"(s2), "r"(m2));
     }
   }
-  return make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
-                    __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
+  out[0] = __byte_perm(v[0], v[1], 0x5410);
+  out[1] = __byte_perm(v[2], v[3], 0x5410);
+  out[2] = __byte_perm(v[0], v[1], 0x7632);
+  out[3] = __byte_perm(v[2], v[3], 0x7632);
 }
 
-template <int kD, bool kBF16>
+template <int kD, bool kBF16, bool kLong>
 __global__ void __launch_bounds__(kThreads) cache4_read_kernel(const Cache4Params p) {
   using T = Tile<kD>;
-  const int b = blockIdx.x / (p.n_tiles * p.n_sides);
-  const int rest = blockIdx.x - b * (p.n_tiles * p.n_sides);
-  const int token0 = (rest / p.n_sides) << p.tile_shift;
-  const int side0 = (rest % p.n_sides) * (T::kTile >> p.tile_shift);
-  const NewRows fresh = new_rows(p.c, b, p.seq_len);
+  const Place<kD, kLong> at(p);
+  const NewRows fresh = new_rows(p.c, at.b, p.seq_len);
   const int lane = threadIdx.x % T::kLanes;
-  uint32_t word[kUnroll], params[kUnroll];
+  uint2 word[kUnroll];
+  uint32_t params[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int r = u * T::kRows + threadIdx.x / T::kLanes;
-    const int token = token0 + (r & ((1 << p.tile_shift) - 1)), side = side0 + (r >> p.tile_shift);
-    word[u] = params[u] = 0;
-    if (token < fresh.count && side < 2 * p.c.n_kv_heads) {
-      const int64_t at = cache_row<kD>(p, b, fresh.first + token, side);
-      if (at >= 0) {
-        const char* row = static_cast<const char*>(p.c.cache) + at;
-        word[u] = *reinterpret_cast<const uint32_t*>(row + lane * 4);
-        params[u] = *reinterpret_cast<const uint32_t*>(row + kD / 2 + lane / 8 * 4);
+    const int token = at.token(p, u), side = at.side(p, u);
+    word[u] = make_uint2(0, 0);
+    params[u] = 0;
+    if (token < fresh.count && (kLong || side < 2 * p.c.n_kv_heads)) {
+      const char* row = cache_row<kD>(p, at.b, fresh.first + token, side);
+      if (row != nullptr) {
+        if constexpr (kD == 128) {
+          word[u] = *reinterpret_cast<const uint2*>(row + lane * 8);
+        } else {  // rows of 36 bytes
+          word[u].x = *reinterpret_cast<const uint32_t*>(row + lane * 8);
+          word[u].y = *reinterpret_cast<const uint32_t*>(row + lane * 8 + 4);
+        }
+        params[u] = *reinterpret_cast<const uint32_t*>(row + kD / 2 + lane / 4 * 4);
       }
     }
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int r = u * T::kRows + threadIdx.x / T::kLanes;
-    const int token = token0 + (r & ((1 << p.tile_shift) - 1)), side = side0 + (r >> p.tile_shift);
-    if (token < p.seq_len && side < 2 * p.c.n_kv_heads) {
-      const int w = side & 1;
-      char* dst = p.x[w] + b * p.x_s[w][0] + token * p.x_s[w][1] + (side >> 1) * p.x_s[w][2] + lane * 16;
-      *reinterpret_cast<uint4*>(dst) = dequantise8<kBF16>(word[u], params[u]);
+    const int token = at.token(p, u), side = at.side(p, u);
+    if (token < p.seq_len && (kLong || side < 2 * p.c.n_kv_heads)) {
+      const uint32_t s2 = __byte_perm(params[u], 0, 0x1010), m2 = __byte_perm(params[u], 0, 0x3232);
+      uint32_t v[2][4];
+      dequantise8<kBF16>(v[0], word[u].x, s2, m2);
+      dequantise8<kBF16>(v[1], word[u].y, s2, m2);
+      store32(outer_row<kD>(p, at.b, token, side), v);
     }
   }
 }
@@ -303,17 +385,25 @@ int cache4_move(const AfaCache4* c, const void* k, const void* v, const int64_t*
   const unsigned g = static_cast<unsigned>(grid);
   const auto s = static_cast<cudaStream_t>(stream);
   const bool bf = c->dtype == AFA_DTYPE_BF16;
-#define AFA_MOVE(D, BF)                                             \
-  if (kWrite)                                                       \
-    cache4_write_kernel<D, BF><<<g, kThreads, 0, s>>>(p);           \
-  else                                                              \
-    cache4_read_kernel<D, BF><<<g, kThreads, 0, s>>>(p)
+  const bool one_side = (1 << p.tile_shift) == tile;
+#define AFA_MOVE_AS(D, BF, LONG)                             \
+  if (kWrite)                                                \
+    cache4_write_kernel<D, BF, LONG><<<g, kThreads, 0, s>>>(p); \
+  else                                                       \
+    cache4_read_kernel<D, BF, LONG><<<g, kThreads, 0, s>>>(p)
+#define AFA_MOVE(D, BF)          \
+  if (one_side) {                \
+    AFA_MOVE_AS(D, BF, true);    \
+  } else {                       \
+    AFA_MOVE_AS(D, BF, false);   \
+  }
   if (c->head_dim == 64) {
-    if (bf) { AFA_MOVE(64, true); } else { AFA_MOVE(64, false); }
+    if (bf) { AFA_MOVE(64, true) } else { AFA_MOVE(64, false) }
   } else {
-    if (bf) { AFA_MOVE(128, true); } else { AFA_MOVE(128, false); }
+    if (bf) { AFA_MOVE(128, true) } else { AFA_MOVE(128, false) }
   }
 #undef AFA_MOVE
+#undef AFA_MOVE_AS
   return ops_launched();
 }
 

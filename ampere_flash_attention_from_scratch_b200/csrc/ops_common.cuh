@@ -79,12 +79,32 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
-__device__ __forceinline__ uint4 ldg_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+// 32 bytes at a time: the row strides and addresses are multiples of 16, so where
+// the address is not one of 32 they go as two halves.
+__device__ __forceinline__ void load32(uint32_t (&v)[2][4], const char* p) {
+  if ((reinterpret_cast<uintptr_t>(p) & 31u) == 0u) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0][0]), "=r"(v[0][1]), "=r"(v[0][2]), "=r"(v[0][3]), "=r"(v[1][0]), "=r"(v[1][1]),
+                   "=r"(v[1][2]), "=r"(v[1][3])
+                 : "l"(p));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(v[i][0]), "=r"(v[i][1]), "=r"(v[i][2]), "=r"(v[i][3])
+                   : "l"(p + 16 * i));
+  }
+}
+__device__ __forceinline__ void store32(char* p, const uint32_t (&v)[2][4]) {
+  if ((reinterpret_cast<uintptr_t>(p) & 31u) == 0u) {
+    asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0][0]), "r"(v[0][1]), "r"(v[0][2]),
+                 "r"(v[0][3]), "r"(v[1][0]), "r"(v[1][1]), "r"(v[1][2]), "r"(v[1][3]), "l"(p)
+                 : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<uint4*>(p + 16 * i) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+  }
 }
 
 // The kernels' report of a bad table entry or length (include/afa_sm100_ops.h).
