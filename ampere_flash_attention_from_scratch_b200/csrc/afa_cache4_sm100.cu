@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kThreads) cache4_write_kernel(const Cache4Para
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[u][i / 4][i % 4] = 0;
     if (token < fresh.count && (kLong || side < 2 * p.c.n_kv_heads)) {
-      load32(x[u], outer_row<kD>(p, at.b, token, side));
+      load32<true>(x[u], outer_row<kD>(p, at.b, token, side));
       row[u] = cache_row<kD>(p, at.b, fresh.first + token, side);
     }
   }

@@ -20,7 +20,8 @@ namespace {
 using namespace afa100;
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // rows a thread has in flight: 8 loads of 16 bytes
+constexpr int kMaxTokens = 16;   // of a CTA
+constexpr int kMaxHeads = 8192;  // q's and k's together
 
 struct RotaryParams {
   const char* in[2];  // q, k
@@ -33,8 +34,17 @@ struct RotaryParams {
   int32_t axis_end[AFA_ROTARY_MAX_AXES];  // first pair behind each axis
   int32_t n_axes, pos_type;
   int32_t seq_len, n_heads, heads_all, head_dim, half;
+  uint32_t heads_magic;      // ceil(2^32 / heads_all): row / heads_all is the high half of row * heads_magic
+                             // (of more than one head; rows < 2^17)
   int32_t n_tokens, tokens;  // all of them, and of one CTA
   int32_t inverse;
+};
+
+// How a thread's channels lie in a row.
+enum Layout {
+  kHalvesWide,    // 16 of one half and the 16 that pair with them: two accesses of 32 bytes
+  kHalvesNarrow,  // 8 and 8: two accesses of 16 bytes, for halves that are not a multiple of 16
+  kNeighbours,    // 16 in a row, pairs side by side: one access of 32 bytes
 };
 
 __device__ __forceinline__ double load_position(const RotaryParams& p, int64_t at) {
@@ -55,14 +65,23 @@ __device__ __forceinline__ float2 cos_sin(double angle) {
   return make_float2(c, s);
 }
 
-// A thread turns 16 channels of a row: channels [8j, 8j + 8) of both halves, or
-// 16 neighbouring ones when pairs are interleaved -- 8 pairs either way -- and
-// copies 16 neighbouring ones behind rot_dim.
-template <bool kBF16, bool kInterleaved>
+// Each thread turns the same channels of several rows (a row: one head of one
+// token), kUnroll of them at a time, and copies the channels behind rot_dim.
+template <bool kBF16, Layout kLayout>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
-  extern __shared__ float2 table[];  // [tokens][half]: cosine, sine
+  constexpr int kPairs = kLayout == kHalvesWide ? 16 : 8;  // of a thread
+  constexpr int kUnroll = kLayout == kHalvesWide ? 2 : 4;  // 128 bytes of loads in flight
+  extern __shared__ float4 table[];  // [tokens][kPairs / 2][blocks of kPairs]: cos, sin, cos, sin
+  __shared__ longlong2 base[kMaxTokens][2];  // a token's first q and k row: in, out
   const int token0 = blockIdx.x * p.tokens;
   const int n_tok = min(p.tokens, p.n_tokens - token0);
+  const int blocks = p.half / kPairs;
+  if (threadIdx.x < 2 * n_tok) {
+    const int t = threadIdx.x >> 1, w = threadIdx.x & 1;
+    const int b = (token0 + t) / p.seq_len, n = (token0 + t) - b * p.seq_len;
+    base[t][w] = make_longlong2(reinterpret_cast<long long>(p.in[w]) + b * p.in_s[w][0] + n * p.in_s[w][1],
+                                reinterpret_cast<long long>(p.out[w]) + b * p.out_s[w][0] + n * p.out_s[w][1]);
+  }
   for (int i = threadIdx.x; i < n_tok * p.half; i += kThreads) {
     const int t = i / p.half, j = i - t * p.half;
     const int b = (token0 + t) / p.seq_len, n = (token0 + t) - b * p.seq_len;
@@ -71,68 +90,88 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
     const double pos = load_position(p, axis * p.pos_s[0] + b * p.pos_s[1] + n * p.pos_s[2]);
     float2 cs = cos_sin(pos * static_cast<double>(p.inv_freq[j]));
     if (p.inverse) cs.y = -cs.y;
-    table[i] = cs;
+    // neighbouring threads read neighbouring blocks: their entries lie side by side
+    reinterpret_cast<float2*>(table + t * (p.half / 2) + j % kPairs / 2 * blocks + j / kPairs)[j & 1] = cs;
   }
   __syncthreads();
 
-  const int per_row = p.head_dim >> 4;
+  const int per_row = p.head_dim / (2 * kPairs);
   const int j = threadIdx.x % per_row;
-  const int rows_step = kThreads / per_row;
-  const bool turned = j < (p.half >> 3);
-  // byte offsets of the thread's two 16-byte pieces within a row
-  const int off0 = kInterleaved || !turned ? j * 32 : j * 16;
-  const int off1 = kInterleaved || !turned ? off0 + 16 : off0 + p.half * 2;
+  const int step = kThreads / per_row;
+  if (threadIdx.x >= step * per_row) return;
+  const bool turned = j < blocks;
+  // byte offsets of the thread's two pieces within a row
+  const int off0 = kLayout == kNeighbours || !turned ? j * 4 * kPairs : j * 2 * kPairs;
+  const int off1 = kLayout == kNeighbours || !turned ? off0 + 2 * kPairs : off0 + p.half * 2;
   const int rows = n_tok * p.heads_all;
-  if (threadIdx.x >= rows_step * per_row) return;
-  for (int r0 = threadIdx.x / per_row; r0 < rows; r0 += rows_step * kUnroll) {
-    uint4 x[kUnroll], y[kUnroll];
+  for (int r0 = threadIdx.x / per_row; r0 < rows; r0 += step * kUnroll) {
+    uint32_t x[kUnroll][kPairs];  // the two pieces
     char* dst[kUnroll];
     int tok[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int r = r0 + u * rows_step;
+      const int r = r0 + u * step;
       dst[u] = nullptr;
       if (r < rows) {
-        const int t = r / p.heads_all, h = r - t * p.heads_all;
-        const int b = (token0 + t) / p.seq_len, n = (token0 + t) - b * p.seq_len;
+        const int t = p.heads_all == 1 ? r : __umulhi(static_cast<uint32_t>(r), p.heads_magic);
+        int h = r - t * p.heads_all;
         const int w = h >= p.n_heads;  // 0: q, 1: k
-        const int hh = w ? h - p.n_heads : h;
-        const char* src = p.in[w] + b * p.in_s[w][0] + n * p.in_s[w][1] + hh * p.in_s[w][2];
-        dst[u] = p.out[w] + b * p.out_s[w][0] + n * p.out_s[w][1] + hh * p.out_s[w][2];
+        if (w) h -= p.n_heads;
+        const longlong2 at = base[t][w];
+        const char* src = reinterpret_cast<const char*>(at.x) + h * p.in_s[w][2];
+        dst[u] = reinterpret_cast<char*>(at.y) + h * p.out_s[w][2];
         tok[u] = t;
-        x[u] = *reinterpret_cast<const uint4*>(src + off0);
-        y[u] = *reinterpret_cast<const uint4*>(src + off1);
+        if constexpr (kLayout == kHalvesWide) {
+          load32<false>(reinterpret_cast<uint32_t(&)[2][4]>(x[u][0]), src + off0);
+          load32<false>(reinterpret_cast<uint32_t(&)[2][4]>(x[u][8]), src + off1);
+        } else if constexpr (kLayout == kNeighbours) {
+          load32<false>(reinterpret_cast<uint32_t(&)[2][4]>(x[u][0]), src + off0);
+        } else {
+          reinterpret_cast<uint4&>(x[u][0]) = *reinterpret_cast<const uint4*>(src + off0);
+          reinterpret_cast<uint4&>(x[u][4]) = *reinterpret_cast<const uint4*>(src + off1);
+        }
       }
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       if (dst[u] == nullptr) continue;
       if (turned) {
-        const float2* cs = table + tok[u] * p.half + j * 8;
-        uint32_t* xs = reinterpret_cast<uint32_t*>(&x[u]);
-        uint32_t* ys = reinterpret_cast<uint32_t*>(&y[u]);
-        if constexpr (kInterleaved) {
+        const float4* cs = table + tok[u] * (p.half / 2) + j;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint32_t& w = i < 4 ? xs[i] : ys[i - 4];
-            const float2 v = unpack2<kBF16>(w);
-            const float2 c = cs[i];
-            w = pack2<kBF16>(v.x * c.x - v.y * c.y, v.y * c.x + v.x * c.y);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 a = unpack2<kBF16>(xs[i]), b = unpack2<kBF16>(ys[i]);
-            const float2 c0 = cs[2 * i], c1 = cs[2 * i + 1];
-            xs[i] = pack2<kBF16>(a.x * c0.x - b.x * c0.y, a.y * c1.x - b.y * c1.y);
-            ys[i] = pack2<kBF16>(b.x * c0.x + a.x * c0.y, b.y * c1.x + a.y * c1.y);
+        for (int i = 0; i < kPairs / 2; ++i) {
+          const float4 c = cs[i * blocks];  // of pairs 2i and 2i + 1
+          if constexpr (kLayout == kNeighbours) {
+            const float2 v = unpack2<kBF16>(x[u][2 * i]), w = unpack2<kBF16>(x[u][2 * i + 1]);
+            x[u][2 * i] = pack2<kBF16>(v.x * c.x - v.y * c.y, v.y * c.x + v.x * c.y);
+            x[u][2 * i + 1] = pack2<kBF16>(w.x * c.z - w.y * c.w, w.y * c.z + w.x * c.w);
+          } else {
+            const float2 a = unpack2<kBF16>(x[u][i]), b = unpack2<kBF16>(x[u][i + kPairs / 2]);
+            x[u][i] = pack2<kBF16>(a.x * c.x - b.x * c.y, a.y * c.z - b.y * c.w);
+            x[u][i + kPairs / 2] = pack2<kBF16>(b.x * c.x + a.x * c.y, b.y * c.z + a.y * c.w);
           }
         }
       }
-      *reinterpret_cast<uint4*>(dst[u] + off0) = x[u];
-      *reinterpret_cast<uint4*>(dst[u] + off1) = y[u];
+      if constexpr (kLayout == kHalvesWide) {
+        store32(dst[u] + off0, reinterpret_cast<uint32_t(&)[2][4]>(x[u][0]));
+        store32(dst[u] + off1, reinterpret_cast<uint32_t(&)[2][4]>(x[u][8]));
+      } else if constexpr (kLayout == kNeighbours) {
+        store32(dst[u] + off0, reinterpret_cast<uint32_t(&)[2][4]>(x[u][0]));
+      } else {
+        *reinterpret_cast<uint4*>(dst[u] + off0) = reinterpret_cast<uint4&>(x[u][0]);
+        *reinterpret_cast<uint4*>(dst[u] + off1) = reinterpret_cast<uint4&>(x[u][4]);
+      }
     }
   }
+}
+
+template <bool kBF16>
+void launch_rotary(Layout layout, unsigned grid, size_t smem, cudaStream_t s, const RotaryParams& p) {
+  if (layout == kNeighbours)
+    rotary_kernel<kBF16, kNeighbours><<<grid, kThreads, smem, s>>>(p);
+  else if (layout == kHalvesWide)
+    rotary_kernel<kBF16, kHalvesWide><<<grid, kThreads, smem, s>>>(p);
+  else
+    rotary_kernel<kBF16, kHalvesNarrow><<<grid, kThreads, smem, s>>>(p);
 }
 
 }  // namespace
@@ -173,7 +212,7 @@ extern "C" int afa_rotary_sm100(const AfaRotaryArgs* a, void* stream) {
     return AFA_ERR_MISALIGNED;
   const int64_t tokens = int64_t{1} * a->batch * a->seq_len;
   const int64_t heads = int64_t{1} * a->n_heads + (has_k ? a->n_k_heads : 0);
-  if (tokens > INT32_MAX - 64 || heads > 65536) return AFA_ERR_TOO_LARGE;
+  if (tokens > INT32_MAX - 64 || heads > kMaxHeads) return AFA_ERR_TOO_LARGE;
 
   int dev = 0, sms = 0;
   const int rc = ops_device(&dev, &sms);
@@ -201,27 +240,24 @@ extern "C" int afa_rotary_sm100(const AfaRotaryArgs* a, void* stream) {
   p.half = a->rot_dim / 2;
   p.n_tokens = static_cast<int32_t>(tokens);
   p.inverse = a->inverse;
-  // Tokens a CTA: as many as give each thread kUnroll rows, unless the GPU would
-  // then have fewer than four CTAs an SM.
-  const int per_row = a->head_dim / 16;
-  int64_t t = (int64_t{kUnroll} * (kThreads / per_row) + heads - 1) / heads;
+  p.heads_magic = static_cast<uint32_t>(((uint64_t{1} << 32) + heads - 1) / heads);
+  const Layout layout = a->interleaved                                             ? kNeighbours
+                        : p.half % 16 == 0 && (a->head_dim - a->rot_dim) % 32 == 0 ? kHalvesWide
+                                                                                   : kHalvesNarrow;
+  // Tokens a CTA: as many as keep each thread busy for two rounds of loads, unless
+  // the GPU would then have fewer than four CTAs an SM.
+  const int rows = layout == kHalvesWide ? 4 * (kThreads / (a->head_dim / 32)) : 8 * (kThreads / (a->head_dim / 16));
+  int64_t t = (rows + heads - 1) / heads;
   const int64_t fill = tokens / (4 * static_cast<int64_t>(sms));
   t = t > fill ? fill : t;
-  t = t < 1 ? 1 : (t > 16 ? 16 : t);
+  t = t < 1 ? 1 : (t > kMaxTokens ? kMaxTokens : t);
   p.tokens = static_cast<int32_t>(t);
   const unsigned grid = static_cast<unsigned>((tokens + t - 1) / t);
   const size_t smem = static_cast<size_t>(t) * p.half * sizeof(float2);  // at most 16 * 256 * 8 = 32 KB
   const auto s = static_cast<cudaStream_t>(stream);
-  if (a->dtype == AFA_DTYPE_BF16) {
-    if (a->interleaved)
-      rotary_kernel<true, true><<<grid, kThreads, smem, s>>>(p);
-    else
-      rotary_kernel<true, false><<<grid, kThreads, smem, s>>>(p);
-  } else {
-    if (a->interleaved)
-      rotary_kernel<false, true><<<grid, kThreads, smem, s>>>(p);
-    else
-      rotary_kernel<false, false><<<grid, kThreads, smem, s>>>(p);
-  }
+  if (a->dtype == AFA_DTYPE_BF16)
+    launch_rotary<true>(layout, grid, smem, s, p);
+  else
+    launch_rotary<false>(layout, grid, smem, s, p);
   return ops_launched();
 }

@@ -80,19 +80,31 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 // 32 bytes at a time: the row strides and addresses are multiples of 16, so where
-// the address is not one of 32 they go as two halves.
+// the address is not one of 32 they go as two halves.  kReadOnly: nothing writes
+// that memory while the kernel runs.
+template <bool kReadOnly>
 __device__ __forceinline__ void load32(uint32_t (&v)[2][4], const char* p) {
   if ((reinterpret_cast<uintptr_t>(p) & 31u) == 0u) {
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(v[0][0]), "=r"(v[0][1]), "=r"(v[0][2]), "=r"(v[0][3]), "=r"(v[1][0]), "=r"(v[1][1]),
-                   "=r"(v[1][2]), "=r"(v[1][3])
-                 : "l"(p));
+    if constexpr (kReadOnly)
+      asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(v[0][0]), "=r"(v[0][1]), "=r"(v[0][2]), "=r"(v[0][3]), "=r"(v[1][0]), "=r"(v[1][1]),
+                     "=r"(v[1][2]), "=r"(v[1][3])
+                   : "l"(p));
+    else
+      asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(v[0][0]), "=r"(v[0][1]), "=r"(v[0][2]), "=r"(v[0][3]), "=r"(v[1][0]), "=r"(v[1][1]),
+                     "=r"(v[1][2]), "=r"(v[1][3])
+                   : "l"(p)
+                   : "memory");
   } else {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(v[i][0]), "=r"(v[i][1]), "=r"(v[i][2]), "=r"(v[i][3])
-                   : "l"(p + 16 * i));
+    for (int i = 0; i < 2; ++i) {
+      const uint4 h = *reinterpret_cast<const uint4*>(p + 16 * i);
+      v[i][0] = h.x;
+      v[i][1] = h.y;
+      v[i][2] = h.z;
+      v[i][3] = h.w;
+    }
   }
 }
 __device__ __forceinline__ void store32(char* p, const uint32_t (&v)[2][4]) {
