@@ -45,8 +45,8 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStep = 32;               // tokens of a warp's step
 constexpr int kUnit = kWarps * kStep;   // tokens of a unit
-constexpr int kStages = 4;              // steps of a warp's ring, one less in flight
-constexpr int kItemUnits = 1;           // units an item is charged beside its tokens'
+constexpr int kStages = 3;              // steps of a warp's ring, one less in flight
+constexpr int kItemUnits = 4;           // units an item is charged beside its tokens'
 constexpr float kRescale = 8.0f;        // log2 units a score may pass the reference maximum by
 constexpr float kHeadroom = 7.0f;       // log2 of p s' at the reference maximum and the largest step
 
@@ -658,10 +658,10 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
                          pick(hi8, 0x000f000fu, 0x800f0000u), pick(hi8, 0x00f000f0u, 0x80f00000u), b0, b1);
               } else {
                 // c' - 8, and 16 times that
-                mma16816(d, sub2((lo8 & 0x000f000fu) | 0x64006400u, 0x64086408u),
-                         sub2((lo8 & 0x00f000f0u) | 0x64006400u, 0x64806480u),
-                         sub2((hi8 & 0x000f000fu) | 0x64006400u, 0x64086408u),
-                         sub2((hi8 & 0x00f000f0u) | 0x64006400u, 0x64806480u), b0, b1);
+                mma16816(d, sub2(pick(lo8, 0x000f000fu, 0x64006400u), 0x64086408u),
+                         sub2(pick(lo8, 0x00f000f0u, 0x64006400u), 0x64806480u),
+                         sub2(pick(hi8, 0x000f000fu, 0x64006400u), 0x64086408u),
+                         sub2(pick(hi8, 0x00f000f0u, 0x64006400u), 0x64806480u), b0, b1);
               }
             }
           }
