@@ -152,6 +152,8 @@ class AfaCache4FwdArgs(ctypes.Structure):
         ("n_heads", ctypes.c_int32),
         ("causal", ctypes.c_int32),
         ("scale", ctypes.c_float),
+        ("timeout_ns", ctypes.c_uint64),
+        ("test_flags", ctypes.c_uint32),
     ]
 
 

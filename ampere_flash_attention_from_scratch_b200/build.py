@@ -103,7 +103,10 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     sources = [
         *units,
         CSRC / "afa_fwd_kernel.cuh",
+        CSRC / "afa_cache4_fwd_common.cuh",
+        CSRC / "afa_cache4_wide_kernel.cuh",
         CSRC / "ops_common.cuh",
+        CSRC / "ops_sites.h",
         CSRC / "sm100_ptx.cuh",
         inc,
         INCLUDE / "afa_sm100.h",

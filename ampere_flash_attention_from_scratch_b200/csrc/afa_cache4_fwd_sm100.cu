@@ -34,8 +34,8 @@
 #include <cmath>
 #include <type_traits>
 
-#include "ops_common.cuh"
-#include "sm100_ptx.cuh"
+#include "afa_cache4_fwd_common.cuh"
+#include "afa_cache4_wide_kernel.cuh"
 
 namespace {
 
@@ -44,43 +44,9 @@ using namespace afa100;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStep = 32;               // tokens of a warp's step
-constexpr int kUnit = kWarps * kStep;   // tokens of a unit
+static_assert(kUnit == kWarps * kStep, "a unit is one step of every warp");
 constexpr int kStages = 3;              // steps of a warp's ring, one less in flight
-constexpr int kItemUnits = 4;           // units an item is charged beside its tokens'
-constexpr float kRescale = 8.0f;        // log2 units a score may pass the reference maximum by
-constexpr float kHeadroom = 7.0f;       // log2 of p s' at the reference maximum and the largest step
 
-struct FwdParams4 {
-  AfaCache4 c;
-  const char* q;
-  char* o;
-  int64_t q_s[3];  // bytes: batch, seq, head
-  int64_t o_s[3];
-  float* lse;
-  float* ws;
-  int32_t seq_len, n_heads, group;
-  int32_t rows;       // seq_len * group query rows of a key/value head
-  int32_t row_tiles;  // blocks of kRows of them
-  int32_t page_shift;
-  uint32_t page_stride;
-  int32_t causal;
-  float scale_log2;
-};
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-// p + n * stride bytes
-__device__ __forceinline__ const char* far(const char* p, uint32_t n, uint32_t stride) {
-  uint64_t r;
-  asm("mad.wide.u32 %0, %1, %2, %3;" : "=l"(r) : "r"(n), "r"(stride), "l"(reinterpret_cast<uint64_t>(p)));
-  return reinterpret_cast<const char*>(r);
-}
 __device__ __forceinline__ uint32_t lds32(const char* a) { return *reinterpret_cast<const uint32_t*>(a); }
 __device__ __forceinline__ uint2 lds64(const char* a) { return *reinterpret_cast<const uint2*>(a); }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -129,121 +95,6 @@ __device__ __forceinline__ float sum_over_rows(float v) {
 }
 
 // ---------------------------------------------------------------------------
-// The division of the work, formed alike by every warp of both kernels
-// ---------------------------------------------------------------------------
-
-// Tokens of sequence b, 0 (reported) where the lengths are not possible.
-__device__ __forceinline__ int tokens_of(const FwdParams4& p, int b) {
-  const int kv = p.c.kv_lens[b];
-  const int fresh = p.c.new_lens != nullptr ? p.c.new_lens[b] : p.seq_len;
-  if (kv < 0 || kv > p.c.max_pages * p.c.page_size || fresh < 0 || fresh > p.seq_len) {
-    report(p.c.status, AFA_DEV_BAD_LENGTH);
-    return 0;
-  }
-  return kv;
-}
-// Units of an item: kItemUnits that stand for what starting and ending an item
-// costs, then those of its tokens (one at least).
-__device__ __forceinline__ int units_of(int tokens) {
-  return kItemUnits + (tokens <= kUnit ? 1 : (tokens + kUnit - 1) / kUnit);
-}
-
-struct Division {
-  int ctas;  // CTAs that share the units: the first `more` of them take each + 1, the others `each`
-  int each, more;
-  // First unit of CTA i.
-  __device__ __forceinline__ int first(int i) const { return i * each + min(i, more); }
-  // The CTA that holds unit u.
-  __device__ __forceinline__ int holder(int u) const {
-    const int longer = more * (each + 1);
-    return u < longer ? u / (each + 1) : more + (u - longer) / each;
-  }
-};
-
-// Sum of units over this lane's share of the sequences, a contiguous range of
-// `per` of them, and from it the division.  The host has made sure that the
-// units of the call fit 31 bits.
-__device__ __forceinline__ Division divide(const FwdParams4& p, int per, int grid, int* before_lane) {
-  const int lane = static_cast<int>(threadIdx.x & 31u);
-  int mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int b = lane * per + i;
-    if (b < p.c.batch) mine += units_of(tokens_of(p, b));
-  }
-  mine *= p.c.n_kv_heads * p.row_tiles;
-  int upto = mine;
-#pragma unroll
-  for (int i = 1; i < 32; i <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, upto, i);
-    if (lane >= i) upto += v;
-  }
-  *before_lane = upto - mine;
-  const int total = __shfl_sync(0xffffffffu, upto, 31);
-  Division d;
-  d.ctas = min(total, grid);
-  d.each = total / d.ctas;
-  d.more = total - d.each * d.ctas;
-  return d;
-}
-
-struct Item {
-  int b;      // sequence
-  int which;  // key/value head * row_tiles + row block
-  int unit;   // unit within the item
-  int units;
-  int tokens;
-};
-
-// The item that unit u belongs to.
-__device__ __forceinline__ Item find_item(const FwdParams4& p, int per, int before_lane, int u) {
-  const int items = p.c.n_kv_heads * p.row_tiles;
-  const unsigned owners = __ballot_sync(0xffffffffu, before_lane <= u);
-  const int owner = 31 - __clz(owners);
-  int left = u - __shfl_sync(0xffffffffu, before_lane, owner);
-  // lanes behind the last sequence own nothing and start where it ends: u is below that
-  Item it;
-  it.b = owner * per;
-  for (;;) {
-    it.tokens = tokens_of(p, it.b);
-    it.units = units_of(it.tokens);
-    const int here = it.units * items;
-    if (left < here || it.b + 1 >= p.c.batch) break;
-    left -= here;
-    ++it.b;
-  }
-  it.which = left / it.units;
-  it.unit = left - it.which * it.units;
-  return it;
-}
-
-// A CTA's walk through its units, piece by piece (a piece: its part of one item).
-struct Walk {
-  Item it;
-  int left;      // units of the CTA from this piece on
-  int unit_end;  // end of the piece within the item
-  int tok, tok_end;
-  __device__ __forceinline__ void open(int warp) {
-    unit_end = it.unit + left < it.units ? it.unit + left : it.units;
-    tok = max(it.unit - kItemUnits, 0) * kUnit + warp * kStep;
-    tok_end = min(it.tokens, max(unit_end - kItemUnits, 0) * kUnit);
-  }
-  // To the next piece; false at the end of the CTA's units.
-  __device__ __forceinline__ bool next(const FwdParams4& p, int warp) {
-    left -= unit_end - it.unit;
-    if (left <= 0) return false;
-    it.unit = 0;
-    if (++it.which == p.c.n_kv_heads * p.row_tiles) {
-      it.which = 0;
-      ++it.b;
-      it.tokens = tokens_of(p, it.b);
-      it.units = units_of(it.tokens);
-    }
-    open(warp);
-    return true;
-  }
-};
-
-// ---------------------------------------------------------------------------
 // Attention
 // ---------------------------------------------------------------------------
 template <int kD, int kNT>
@@ -284,12 +135,12 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
     if (cta >= div.ctas) return;
     w.it = find_item(p, per, before_lane, div.first(cta));
     w.left = div.first(cta + 1) - div.first(cta);
-    w.open(warp);
+    w.open(warp * kStep);
   }
   // Past pieces that are only the cost of an item whose tokens another CTA has; false at the end.
   auto skip_empty = [&](Walk& walk) {
     bool go = true;
-    while (go && walk.unit_end <= kItemUnits) go = walk.next(p, warp);
+    while (go && walk.unit_end <= kItemUnits) go = walk.next(p, warp * kStep);
     return go;
   };
 
@@ -332,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
   };
   // To the next piece with tokens for this warp, if the loads have reached the end of theirs.
   auto settle = [&]() {
-    while (more && ahead.tok >= ahead.tok_end) more = ahead.next(p, warp);
+    while (more && ahead.tok >= ahead.tok_end) more = ahead.next(p, warp * kStep);
     if (more) {
       const int head = ahead.it.which / p.row_tiles;
       side = static_cast<const char*>(p.c.cache) + static_cast<int64_t>(head) * 2 * p.c.page_size * kRow + lane * 16;
@@ -686,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(
     }
     __syncwarp();
 
-    const bool go = w.next(p, warp) && skip_empty(w);
+    const bool go = w.next(p, warp * kStep) && skip_empty(w);
     if (go) load_queries();
 
     // --- the warps' shares -> the CTA's -------------------------------------------------------------------
@@ -834,7 +685,7 @@ __global__ void __launch_bounds__(128) cache4_join_kernel(const FwdParams4 p) {
 // Host side
 // ---------------------------------------------------------------------------
 struct Kernel4 {
-  int rows, smem, share_floats;
+  int rows, share_floats;
   cudaError_t (*prepare)(int* ctas_per_sm);
   cudaError_t (*launch)(const FwdParams4&, unsigned grid, cudaStream_t);
 };
@@ -850,10 +701,9 @@ cudaError_t prepare4(int* ctas_per_sm) {
 }
 
 template <int kD, bool kBF16, int kNT>
-cudaError_t launch4(const FwdParams4& p, unsigned grid, cudaStream_t s) {
+cudaError_t join4(const FwdParams4& p, unsigned grid, cudaStream_t s) {
   using L = FwdLayout4<kD, kNT>;
-  cache4_fwd_kernel<kD, kBF16, kNT><<<grid, kThreads, L::kSmem, s>>>(p);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || grid == 1) return e;
   cudaLaunchAttribute overlap{};
   overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -867,18 +717,42 @@ cudaError_t launch4(const FwdParams4& p, unsigned grid, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, cache4_join_kernel<kD, kBF16, kNT>, p);
 }
 
-#define AFA_KERNEL4(D, BF, NT)                                                                                 \
-  {                                                                                                            \
-    FwdLayout4<D, NT>::kRows, FwdLayout4<D, NT>::kSmem, FwdLayout4<D, NT>::kShare,                             \
-        &prepare4<D, BF, NT>, &launch4<D, BF, NT>                                                              \
-  }
-// [head_dim 64, 128][fp16, bf16][8, 16 rows]
-const Kernel4 kKernels4[2][2][2] = {
-    {{AFA_KERNEL4(64, false, 1), AFA_KERNEL4(64, false, 2)}, {AFA_KERNEL4(64, true, 1), AFA_KERNEL4(64, true, 2)}},
-    {{AFA_KERNEL4(128, false, 1), AFA_KERNEL4(128, false, 2)}, {AFA_KERNEL4(128, true, 1), AFA_KERNEL4(128, true, 2)}}};
+template <int kD, bool kBF16, int kNT>
+cudaError_t launch4(const FwdParams4& p, unsigned grid, cudaStream_t s) {
+  cache4_fwd_kernel<kD, kBF16, kNT><<<grid, kThreads, FwdLayout4<kD, kNT>::kSmem, s>>>(p);
+  return join4<kD, kBF16, kNT>(p, grid, s);
+}
+
+// The kernel for many rows; its shares are those of 16 blocks of 8.
+template <int kD, bool kBF16>
+cudaError_t prepare_wide(int* ctas_per_sm) {
+  using L = WideLayout<kD>;
+  static_assert(L::kShare == FwdLayout4<kD, 16>::kShare && L::kRows == FwdLayout4<kD, 16>::kRows, "one join for both");
+  // By design two CTAs an SM, in registers, shared and tensor memory.  (The occupancy query answers 1 for a kernel
+  // that allocates tensor memory.)
+  *ctas_per_sm = 2;
+  return cudaFuncSetAttribute(cache4_wide_kernel<kD, kBF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+}
+
+template <int kD, bool kBF16>
+cudaError_t launch_wide(const FwdParams4& p, unsigned grid, cudaStream_t s) {
+  using L = WideLayout<kD>;
+  cache4_wide_kernel<kD, kBF16><<<grid, L::kThreads, L::kSmem, s>>>(p);
+  return join4<kD, kBF16, 16>(p, grid, s);
+}
+
+#define AFA_KERNEL4(D, BF, NT) \
+  { FwdLayout4<D, NT>::kRows, FwdLayout4<D, NT>::kShare, &prepare4<D, BF, NT>, &launch4<D, BF, NT> }
+#define AFA_WIDE4(D, BF) \
+  { WideLayout<D>::kRows, WideLayout<D>::kShare, &prepare_wide<D, BF>, &launch_wide<D, BF> }
+#define AFA_ROWS4(D, BF) \
+  { AFA_KERNEL4(D, BF, 1), AFA_KERNEL4(D, BF, 2), AFA_WIDE4(D, BF) }
+// [head_dim 64, 128][fp16, bf16][8, 16, 128 rows]
+const Kernel4 kKernels4[2][2][3] = {{AFA_ROWS4(64, false), AFA_ROWS4(64, true)},
+                                    {AFA_ROWS4(128, false), AFA_ROWS4(128, true)}};
 
 std::mutex g_mu4;
-int g_ctas_per_sm[kOpsMaxDevices][2][2][2] = {};
+int g_ctas_per_sm[kOpsMaxDevices][2][2][3] = {};
 
 // Kernel, grid and row blocks of a call.
 int plan4(const AfaCache4* c, int32_t seq_len, int32_t n_heads, const Kernel4** kernel, int32_t* grid,
@@ -888,7 +762,10 @@ int plan4(const AfaCache4* c, int32_t seq_len, int32_t n_heads, const Kernel4** 
   if (seq_len <= 0 || n_heads <= 0 || n_heads % c->n_kv_heads != 0) return AFA_ERR_INVALID_ARGUMENT;
   const int64_t rows = int64_t{seq_len} * (n_heads / c->n_kv_heads);
   if (rows > INT32_MAX - 64) return AFA_ERR_TOO_LARGE;
-  const int di = c->head_dim == 128, ti = c->dtype == AFA_DTYPE_BF16, ni = rows > 8;
+  // mma.sync takes 51 us for every 16 rows of [16 sequences of 512..16384 tokens, 8 key/value heads, 128] fp16,
+  // tcgen05 181 us for 64 rows and 240 us for 128 (d 64: 30, 128 and 175); below about 1000 tokens a sequence the
+  // second starts and ends more slowly (34 us against 21 at one sequence of 2000 tokens, 64 rows).
+  const int di = c->head_dim == 128, ti = c->dtype == AFA_DTYPE_BF16, ni = rows > 64 ? 2 : rows > 8;
   const Kernel4& k = kKernels4[di][ti][ni];
   const int64_t tiles = (rows + k.rows - 1) / k.rows;
   if (c->n_pages > 1 && c->page_stride > UINT32_MAX) return AFA_ERR_TOO_LARGE;
@@ -968,6 +845,8 @@ int afa_cache4_fwd_sm100(const AfaCache4* cache, const AfaCache4FwdArgs* a, void
   p.page_shift = ops_log2(cache->page_size);
   p.page_stride = static_cast<uint32_t>(cache->page_stride);
   p.causal = a->causal;
+  p.timeout_ns = a->timeout_ns != 0 ? a->timeout_ns : 4000000000ull;
+  p.test_flags = a->test_flags;
   const double scale = a->scale > 0.f ? a->scale : 1.0 / (cache->head_dim == 64 ? 8.0 : 11.313708498984761);
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   if (k->launch(p, static_cast<unsigned>(grid), static_cast<cudaStream_t>(stream)) != cudaSuccess) {

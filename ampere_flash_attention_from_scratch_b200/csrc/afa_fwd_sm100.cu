@@ -27,6 +27,7 @@
 #include "afa_fwd_kernel.cuh"
 #include "afa_sm100.h"
 #include "afa_sm100_ops.h"
+#include "ops_sites.h"
 
 namespace {
 
@@ -308,6 +309,13 @@ const char* afa_status_string(int32_t status) {
     case afa100::kSiteCorrAlpha: return "timeout: correction warp waiting for row scale factors";
     case afa100::kSiteCorrStats: return "timeout: correction warp waiting for the final row sums";
     case afa100::kSiteMmaOFree: return "timeout: MMA waiting for the previous item's O to be read out";
+    case afa100::kSiteWideQ: return "timeout: cache MMA waiting for the Q tile";
+    case afa100::kSiteWideKFull: return "timeout: cache MMA waiting for a K tile";
+    case afa100::kSiteWideVFull: return "timeout: cache MMA or softmax waiting for a V tile";
+    case afa100::kSiteWideS: return "timeout: cache softmax or loads waiting for S";
+    case afa100::kSiteWideP: return "timeout: cache MMA waiting for P";
+    case afa100::kSiteWidePv: return "timeout: cache loads or epilogue waiting for O";
+    case afa100::kSiteWideDrain: return "timeout: draining outstanding cache MMAs at exit";
     default: return "unknown device status";
   }
 }

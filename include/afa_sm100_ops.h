@@ -9,6 +9,7 @@
  * As in afa_sm100.h: plain C types, device pointers, a cudaStream_t passed as
  * void*; no call allocates, frees or synchronises; every entry point returns
  * an AFA_* code, checks its arguments before any CUDA call and never throws.
+ * Every wait inside a kernel is bounded, as there.
  *
  * The cache.  One uint8 array [n_pages][n_kv_heads][2][page_size][row] (index
  * 2: keys, values), row = head_dim / 2 + head_dim / 16 bytes: 36 at head_dim
@@ -136,6 +137,9 @@ typedef struct AfaCache4FwdArgs {
   int32_t n_heads;
   int32_t causal;
   float scale; /* <= 0 selects 1/sqrt(head_dim) */
+  uint64_t timeout_ns; /* bound of every device-side wait; 0 selects the default (4 s) */
+  uint32_t test_flags; /* 0 in normal use; AFA_TEST_PRODUCER_IDLE: in calls of more than 16 query rows a
+                          key/value head nothing is loaded, and the bounded waits run out */
 } AfaCache4FwdArgs;
 
 /* Bytes of workspace a call with these sizes needs on the current device, or

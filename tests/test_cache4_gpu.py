@@ -246,6 +246,14 @@ ATTEND = [
     ([2, 1], 4, None, 2, 2, 64, 16, True, torch.float16),  # fewer tokens than rows: rows that see none
     ([130], 33, None, 4, 2, 128, 64, True, torch.float16),  # several row blocks
     ([4100], 1, None, 2, 2, 64, 128, False, torch.bfloat16),
+    # more than 64 rows a key/value head
+    ([600, 64, 0, 63], 17, [17, 17, 0, 5], 8, 2, 128, 16, True, torch.bfloat16),
+    ([65, 1000], 33, None, 8, 2, 64, 32, False, torch.float16),
+    ([300, 40], 40, None, 4, 1, 128, 64, True, torch.float16),  # two tiles, the second of 32 rows; fewer tokens than rows
+    ([777], 129, None, 1, 1, 64, 256, True, torch.bfloat16),
+    ([1, 2, 500], 10, None, 8, 1, 128, 128, False, torch.bfloat16),
+    ([0, 0], 70, None, 1, 1, 64, 16, False, torch.float16),
+    ([2100], 24, None, 6, 2, 128, 32, True, torch.float16),
 ]
 
 
@@ -264,10 +272,10 @@ def test_attention_against_oracle(case):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("d", [64, 128])
 def test_random_shapes(d, dtype):
-    g = torch.Generator().manual_seed(d + (dtype == torch.float16))
+    g = torch.Generator().manual_seed(d + (dtype == torch.float16))  # up to 9 x 14 rows
     r = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))
     for trial in range(12):
-        B, n, HK = r(1, 5), r(1, 6), r(1, 4)
+        B, n, HK = r(1, 5), r(1, 14), r(1, 4)
         H = HK * r(1, 9)
         lens = [r(0, 900) for _ in range(B)]
         new = [r(0, n) for _ in range(B)] if r(0, 1) else None
@@ -286,7 +294,8 @@ def test_ranges(dtype, k_scale, v_scale, q_scale):
     check_attention(q, cache, table, lens, True)
 
 
-def test_rising_maximum_and_steps():
+@pytest.mark.parametrize("n", [1, 50])
+def test_rising_maximum_and_steps(n):
     # scores and values' steps that grow along the sequence: the references move on every step
     lens, d, page = [640], 64, 64
     table, n_pages = pages(lens, page, 1)
@@ -298,7 +307,7 @@ def test_rising_maximum_and_steps():
     v = (torch.randn(640, d, generator=g) * 2.0 ** (t[:, None] / 64.0 - 5)).half()
     for w, x in ((0, k), (1, v)):
         cache[table[0, t // page].long(), 0, w, t % page] = oc.pack_rows(*oc.quantise64(x, torch.float16), torch.float16)
-    q = torch.stack([u, -u, 0 * u]).half().view(1, 1, 3, d)
+    q = torch.stack([u, -u, 0 * u]).half().view(1, 1, 3, d).expand(1, n, 3, d) * torch.linspace(1, 0.1, n).half().view(1, n, 1, 1)
     check_attention(q, cache, table, lens, False)
 
 
@@ -311,19 +320,20 @@ def test_softmax_scale_and_lse_optional():
     assert none is None and torch.equal(o, fa.forward_cache4(*dev, return_lse=True)[0])
 
 
-def test_nan_in_masked_places_stays_there():
+@pytest.mark.parametrize("n", [4, 45])
+def test_nan_in_masked_places_stays_there(n):
     # NaN keys and values behind a row's position must not reach it; a visible one must
-    lens, n = [50], 4
+    lens = [50]
     cache, table = filled(lens, 1, 128, 16, torch.float16, seed=3)
     q = torch.randn(1, n, 2, 128, generator=torch.Generator().manual_seed(1)).half()
     clean, _ = check_attention(q, cache, table, lens, True)
     for side in (0, 1):
         bad = cache.clone()
-        bad[table[0, 48 // 16], 0, side, 48 % 16, 64:] = 255  # token 48: rows 2 and 3 see it
+        bad[table[0, 48 // 16], 0, side, 48 % 16, 64:] = 255  # token 48: the last two rows see it
         o, _ = fa.forward_cache4(q.cuda(), bad.cuda(), table.cuda(), ints(lens).cuda(), None, True)
         fa.check_status(0)
-        assert torch.equal(o[:, :2].cpu().double(), clean[:, :2])
-        assert torch.isnan(o[:, 2:]).all()
+        assert torch.equal(o[:, :-2].cpu().double(), clean[:, :-2])
+        assert torch.isnan(o[:, -2:]).all()
 
 
 def test_negative_steps_are_taken_as_written():
@@ -436,6 +446,42 @@ def test_refusals():
         with pytest.raises(RuntimeError, match=match):
             a(**over)
     fa.check_status(0)
+
+
+def test_wait_that_runs_out_is_reported():
+    # nothing is loaded: the waits of the kernel for many rows run out, the context stays usable
+    import ctypes
+
+    from ampere_flash_attention_from_scratch_b200 import _abi
+
+    lib = _abi.load()
+    cache, table = filled([300, 70], 2, 128, 32, torch.float16, seed=11)
+    q = torch.randn(2, 40, 4, 128, generator=torch.Generator().manual_seed(1)).half()
+    qd, cd, td, ld = q.cuda(), cache.cuda(), table.cuda(), ints([300, 70]).cuda()
+    o, lse = torch.zeros_like(qd), torch.zeros(2, 4, 40, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    c = _abi.AfaCache4()
+    c.cache, c.page_stride, c.page_table, c.table_stride = cd.data_ptr(), cd.stride(0), td.data_ptr(), td.stride(0)
+    c.kv_lens, c.status = ld.data_ptr(), status.data_ptr()
+    c.n_pages, c.page_size, c.max_pages, c.batch, c.n_kv_heads, c.head_dim = cd.shape[0], 32, td.shape[1], 2, 2, 128
+    c.dtype = _abi.AFA_DTYPE_FP16
+    a = _abi.AfaCache4FwdArgs()
+    bytes_ = lib.afa_cache4_fwd_workspace(ctypes.byref(c), 40, 4)
+    ws = torch.empty(bytes_, dtype=torch.uint8, device="cuda")
+    a.q, a.o, a.lse, a.workspace, a.workspace_bytes = qd.data_ptr(), o.data_ptr(), lse.data_ptr(), ws.data_ptr(), bytes_
+    a.q_strides[:] = a.o_strides[:] = [qd.stride(0), qd.stride(1), qd.stride(2)]
+    a.seq_len, a.n_heads, a.causal = 40, 4, 1
+    stream = torch.cuda.current_stream().cuda_stream
+    a.timeout_ns, a.test_flags = 20_000_000, _abi.AFA_TEST_PRODUCER_IDLE
+    assert lib.afa_cache4_fwd_sm100(ctypes.byref(c), ctypes.byref(a), stream) == _abi.AFA_OK
+    torch.cuda.synchronize()
+    assert b"timeout: cache" in lib.afa_status_string(int(status.item()))
+    status.zero_()
+    a.timeout_ns, a.test_flags = 0, 0
+    assert lib.afa_cache4_fwd_sm100(ctypes.byref(c), ctypes.byref(a), stream) == _abi.AFA_OK
+    torch.cuda.synchronize()
+    assert int(status.item()) == 0
+    check_attention(q, cache, table, [300, 70], True, got=(o, lse))
 
 
 # --- streams, graphs, several calls ----------------------------------------------------------------------
