@@ -14,6 +14,7 @@
 // synchronises; what a call needs besides its outputs comes from torch's
 // allocator on the call's stream, so calls and captured graphs never share it.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime.h>
 #include <torch/extension.h>
@@ -58,9 +59,14 @@ void fill_strides(int64_t (&s)[3], const at::Tensor& t) {
   for (int d = 0; d < 3; ++d) s[d] = t.stride(d);
 }
 
+// A new contiguous tensor on `dev`, past the dispatcher (0.3 us of host time less; a call takes 6 to 10).
+at::Tensor fresh_tensor(at::IntArrayRef shape, at::ScalarType type, const at::Device& dev) {
+  return at::Tensor(at::detail::empty_cuda(shape, type, dev, std::nullopt));
+}
+
 // `out` if given (checked against `like`), else a new contiguous tensor.
 at::Tensor output_like(const std::optional<at::Tensor>& out, const at::Tensor& like, const char* name) {
-  if (!out.has_value() || !out->defined()) return at::empty_like(like, at::MemoryFormat::Contiguous);
+  if (!out.has_value() || !out->defined()) return fresh_tensor(like.sizes(), like.scalar_type(), like.device());
   const at::Tensor& o = out.value();
   TORCH_CHECK(o.device().is_cuda(), name, " must be a CUDA tensor");
   TORCH_CHECK(o.dim() == 4 && o.stride(3) == 1, name,
@@ -130,8 +136,8 @@ void rotary_launch(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q
 variable_list rotary_new(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
                          const at::Tensor& inv_freq, const RotaryPlan& plan) {
   c10::cuda::CUDAGuard guard{q.device()};
-  at::Tensor q_out = at::empty_like(q, at::MemoryFormat::Contiguous);
-  at::Tensor k_out = k.defined() ? at::empty_like(k, at::MemoryFormat::Contiguous) : at::Tensor();
+  at::Tensor q_out = fresh_tensor(q.sizes(), q.scalar_type(), q.device());
+  at::Tensor k_out = k.defined() ? fresh_tensor(k.sizes(), k.scalar_type(), k.device()) : at::Tensor();
   rotary_launch(q, k, q_out, k_out, positions, inv_freq, plan);
   return {q_out, k_out};
 }
@@ -374,7 +380,7 @@ std::tuple<at::Tensor, at::Tensor> cache4_read(const at::Tensor& cache, const at
                                  dtype == at::kHalf ? AFA_DTYPE_FP16 : AFA_DTYPE_BF16);
   auto make = [&](const std::optional<at::Tensor>& out, const char* name) {
     const std::vector<int64_t> shape = {batch, n, c.n_kv_heads, c.head_dim};
-    if (!out.has_value() || !out->defined()) return at::empty(shape, at::TensorOptions().dtype(dtype).device(cache.device()));
+    if (!out.has_value() || !out->defined()) return fresh_tensor(shape, dtype, cache.device());
     const at::Tensor& o = *out;
     TORCH_CHECK(o.device() == cache.device() && o.scalar_type() == dtype && o.dim() == 4 && o.sizes() == at::IntArrayRef(shape) &&
                     o.stride(3) == 1,
@@ -418,10 +424,10 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> forward_cache4(
   const int32_t n = static_cast<int32_t>(q.size(1)), heads = static_cast<int32_t>(q.size(2));
   std::optional<at::Tensor> lse;
   if (return_lse)
-    lse = at::empty({q.size(0), q.size(2), q.size(1)}, at::TensorOptions().dtype(at::kFloat).device(q.device()));
+    lse = fresh_tensor({q.size(0), q.size(2), q.size(1)}, at::kFloat, q.device());
   const int64_t bytes = afa_cache4_fwd_workspace(&c, n, heads);
   TORCH_CHECK(bytes >= 0, "afa_cache4_fwd_workspace failed: ", afa_strerror(static_cast<int>(-bytes)));
-  const at::Tensor ws = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(q.device()));
+  const at::Tensor ws = fresh_tensor({bytes}, at::kByte, q.device());
   AfaCache4FwdArgs a{};
   a.q = q.data_ptr();
   a.o = o.data_ptr();
