@@ -153,6 +153,7 @@ struct Walk {
     if (left <= 0) return false;
     it.unit = 0;
     if (++it.which == p.c.n_kv_heads * p.row_tiles) {
+      if (it.b + 1 >= p.c.batch) return false;  // only if the lengths changed under the kernel
       it.which = 0;
       ++it.b;
       it.tokens = tokens_of(p, it.b);

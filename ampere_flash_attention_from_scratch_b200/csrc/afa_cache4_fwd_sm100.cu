@@ -114,7 +114,7 @@ struct FwdLayout4 {
 };
 
 template <int kD, bool kBF16, int kNT>
-__global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) cache4_fwd_kernel(const FwdParams4 p) {
+__global__ void __launch_bounds__(kThreads, kNT == 1 || kD == 64 ? 3 : 2) cache4_fwd_kernel(const FwdParams4 p) {
   using L = FwdLayout4<kD, kNT>;
   constexpr int kG = L::kGroups;
   constexpr int kRow = L::kRow;

@@ -21,7 +21,6 @@ using namespace afa100;
 
 constexpr int kThreads = 256;
 constexpr int kMaxTokens = 16;   // of a CTA
-constexpr int kMaxHeads = 8192;  // q's and k's together
 
 struct RotaryParams {
   const char* in[2];  // q, k
@@ -212,7 +211,7 @@ extern "C" int afa_rotary_sm100(const AfaRotaryArgs* a, void* stream) {
     return AFA_ERR_MISALIGNED;
   const int64_t tokens = int64_t{1} * a->batch * a->seq_len;
   const int64_t heads = int64_t{1} * a->n_heads + (has_k ? a->n_k_heads : 0);
-  if (tokens > INT32_MAX - 64 || heads > kMaxHeads) return AFA_ERR_TOO_LARGE;
+  if (tokens > INT32_MAX - 64 || heads > AFA_ROTARY_MAX_HEADS) return AFA_ERR_TOO_LARGE;
 
   int dev = 0, sms = 0;
   const int rc = ops_device(&dev, &sms);

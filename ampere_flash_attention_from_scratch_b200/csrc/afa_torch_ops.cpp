@@ -64,6 +64,9 @@ at::Tensor fresh_tensor(at::IntArrayRef shape, at::ScalarType type, const at::De
   return at::Tensor(at::detail::empty_cuda(shape, type, dev, std::nullopt));
 }
 
+// A tensor of the caller's has been written: autograd notices if it had saved it.
+void written(const at::Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+
 // `out` if given (checked against `like`), else a new contiguous tensor.
 at::Tensor output_like(const std::optional<at::Tensor>& out, const at::Tensor& like, const char* name) {
   if (!out.has_value() || !out->defined()) return fresh_tensor(like.sizes(), like.scalar_type(), like.device());
@@ -218,6 +221,8 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> rotary(const at::Tensor& q, co
   TORCH_CHECK(inv_freq.dim() == 1 && inv_freq.scalar_type() == at::kFloat && inv_freq.is_contiguous(),
               "inv_freq must be a contiguous 1-D float32 tensor");
   const int64_t axes = positions.size(0), pairs = inv_freq.size(0), d = q.size(3);
+  TORCH_CHECK(q.size(2) + (k.defined() ? k.size(2) : 0) <= AFA_ROTARY_MAX_HEADS, "at most ", AFA_ROTARY_MAX_HEADS,
+              " query and key heads together");
   TORCH_CHECK(axes >= 1 && axes <= AFA_ROTARY_MAX_AXES, "positions must have 1 to ", AFA_ROTARY_MAX_AXES, " axes");
   TORCH_CHECK(d % 16 == 0 && d <= 512, "head_dim must be a multiple of 16 and at most 512 (got ", d, ")");
   TORCH_CHECK(pairs > 0 && pairs % 8 == 0 && 2 * pairs <= d,
@@ -253,6 +258,8 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> rotary(const at::Tensor& q, co
     TORCH_CHECK(!grad || !(q_out.requires_grad() || (k_out.defined() && k_out.requires_grad())),
                 "q_out and k_out must not require a gradient");
     rotary_launch(q, k, q_out, k_out, positions, inv_freq, plan);
+    written(q_out);
+    if (k_out.defined()) written(k_out);
     out = {q_out, k_out};
   } else {
     out = rotary_any(q, k, positions, inv_freq, plan);
@@ -359,6 +366,7 @@ void cache4_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ca
   const int rc = afa_cache4_write_sm100(&c, k.data_ptr(), v.data_ptr(), ks, vs, static_cast<int32_t>(k.size(1)),
                                         at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == AFA_OK, "afa_cache4_write_sm100 failed: ", afa_strerror(rc));
+  written(cache);
 }
 
 std::tuple<at::Tensor, at::Tensor> cache4_read(const at::Tensor& cache, const at::Tensor& page_table,
@@ -394,6 +402,8 @@ std::tuple<at::Tensor, at::Tensor> cache4_read(const at::Tensor& cache, const at
   const int rc = afa_cache4_read_sm100(&c, k.data_ptr(), v.data_ptr(), ks, vs, static_cast<int32_t>(n),
                                        at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == AFA_OK, "afa_cache4_read_sm100 failed: ", afa_strerror(rc));
+  written(k);
+  written(v);
   return std::make_tuple(k, v);
 }
 
@@ -442,6 +452,7 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> forward_cache4(
   a.scale = static_cast<float>(scale);
   const int rc = afa_cache4_fwd_sm100(&c, &a, at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == AFA_OK, "afa_cache4_fwd_sm100 failed: ", afa_strerror(rc));
+  written(o);
   return std::make_tuple(o, lse);
 }
 

@@ -36,6 +36,7 @@ extern "C" {
 #define AFA_POS_INT64 1
 #define AFA_POS_FP32 2
 #define AFA_ROTARY_MAX_AXES 8
+#define AFA_ROTARY_MAX_HEADS 8192 /* n_heads + n_k_heads */
 
 /* Device status words of the cache operators (AfaCache4.status; plain stores,
  * as for afa_fwd_sm100).  What the faulty entry names is skipped: nothing out
@@ -107,14 +108,16 @@ typedef struct AfaCache4 {
  * dtype, code = (x - m) / s rounded to the nearest integer, halves to even, at
  * most 15; 0 where s is 0.  Each rounding is that of the exact quotient.  A
  * group that holds an infinity or a NaN, or whose range passes the largest
- * fp32, gets s = m = NaN and reads back as NaN.  Padding rows are not read and
- * nothing else of the cache is written.  Two sequences of one call must not
- * write the same page. */
+ * fp32, gets s = m = NaN and reads back as NaN.  Padding rows are not written
+ * anywhere and nothing else of the cache is written.  Two sequences of one call
+ * must not write the same row (a page that is in both tables, at the same
+ * place): it would be left with parts of either. */
 int afa_cache4_write_sm100(const AfaCache4* cache, const void* k, const void* v, const int64_t k_strides[3],
                            const int64_t v_strides[3], int32_t seq_len, void* stream);
 
 /* The reverse: k and v rows at the new positions become s * c + m, rounded to
- * dtype; padding rows become zero. */
+ * dtype; padding rows become zero.  (A value within half a step of the type's
+ * largest may round to an infinity.) */
 int afa_cache4_read_sm100(const AfaCache4* cache, void* k, void* v, const int64_t k_strides[3],
                           const int64_t v_strides[3], int32_t seq_len, void* stream);
 
@@ -123,7 +126,11 @@ int afa_cache4_read_sm100(const AfaCache4* cache, void* k, void* v, const int64_
  * unrounded.  n_heads is a multiple of n_kv_heads, grouped as in
  * afa_fwd_sm100.  causal: row i sees the tokens up to its own position
  * kv_lens[b] - new_lens[b] + i.  A row that sees no token and a padding row
- * get O = 0 and lse = -inf. */
+ * get O = 0 and lse = -inf.  A NaN among a row's visible keys makes the row NaN,
+ * one among its visible values the 64 channels of its group; one that is masked
+ * does nothing.  Queries are exact up to 2^110 in magnitude, values' steps up to
+ * 2^100.  Calls of more than 64 query rows a key/value head (seq_len * n_heads /
+ * n_kv_heads) run on tcgen05, others on mma.sync. */
 typedef struct AfaCache4FwdArgs {
   const void* q;
   void* o;
@@ -138,7 +145,7 @@ typedef struct AfaCache4FwdArgs {
   int32_t causal;
   float scale; /* <= 0 selects 1/sqrt(head_dim) */
   uint64_t timeout_ns; /* bound of every device-side wait; 0 selects the default (4 s) */
-  uint32_t test_flags; /* 0 in normal use; AFA_TEST_PRODUCER_IDLE: in calls of more than 16 query rows a
+  uint32_t test_flags; /* 0 in normal use; AFA_TEST_PRODUCER_IDLE: in calls of more than 64 query rows a
                           key/value head nothing is loaded, and the bounded waits run out */
 } AfaCache4FwdArgs;
 

@@ -552,6 +552,27 @@ def test_result_does_not_depend_on_other_sequences_beyond_rounding():
     check_attention(q[2:3], cache, table[2:3], lens[2:3], False)
 
 
+@pytest.mark.parametrize("n", [1, 70])
+def test_many_short_sequences(n):
+    # more sequences than a warp has lanes, a few tokens each, one long among them
+    lens = [(7 * b) % 37 for b in range(1100)]
+    lens[700] = 900
+    cache, table = filled(lens, 1, 64, 16, torch.float16, seed=9)
+    q = torch.randn(1100, n, 1, 64, generator=torch.Generator().manual_seed(3)).half()
+    dev = (q.cuda(), cache.cuda(), table.cuda(), ints(lens).cuda())
+    o, lse = fa.forward_cache4(*dev, return_lse=True)
+    some = [0, 1, 31, 32, 33, 699, 700, 701, 1098, 1099]
+    check_attention(q[some], cache, table[some], [lens[b] for b in some], False, got=(o[some], lse[some]))
+    kr, vr = fa.cache4_read(dev[1], dev[2], dev[3], 900, torch.float16, dev[3])
+    fa.check_status(0)
+    for b in some:
+        rows = oc.sequence_rows(cache, table, b, lens[b])
+        for got, r in ((kr, rows[0]), (vr, rows[1])):
+            c, s, m = oc.unpack_rows(r, torch.float16)
+            want = c * s.repeat_interleave(64, -1) + m.repeat_interleave(64, -1)
+            assert torch.all((got[b, :lens[b]].cpu().double() - want).abs() <= 2.0 ** -11 * want.abs() * 1.001 + 2.0 ** -25)
+
+
 def test_far_pages_pass_32_bit_offsets():
     # a pool of 5 GB: rows near its end are written, read and attended to
     n_pages = 5 * 2 ** 30 // (8 * 2 * 128 * 72)

@@ -189,6 +189,30 @@ def test_capture_of_forward_and_backward():
         assert torch.equal(gx, fa.rotary(dq, None, pos, inv, inverse=True)[0])
 
 
+def test_a_given_output_counts_as_written():
+    # autograd refuses a backward pass through a tensor that was turned in place after it was saved
+    q = torch.ones(1, 2, 1, 64, dtype=torch.float16, device="cuda")
+    w = torch.ones_like(q).requires_grad_()
+    y = (q * w).sum()
+    pos, inv = torch.tensor([[[1, 2]]]).cuda(), _inv(32).cuda()
+    fa.rotary(q, None, pos, inv, q_out=q)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        a, b = fa.rotary(q.clone(), q.clone(), pos, inv)
+        assert torch.equal(a, b)
+
+
+def test_many_heads_and_one():
+    q = torch.randn(1, 2, 3000, 16, generator=torch.Generator().manual_seed(8)).half().cuda()
+    pos, inv = torch.tensor([[[5, 900]]]).cuda(), _inv(8).cuda()
+    a, _ = fa.rotary(q, None, pos, inv)
+    for h in (0, 1499, 2999):
+        assert torch.equal(a[:, :, h:h + 1], fa.rotary(q[:, :, h:h + 1], None, pos, inv)[0])
+    with pytest.raises(RuntimeError, match="heads together"):
+        fa.rotary(q.expand(1, 2, 3000, 16).repeat(1, 1, 3, 1), None, pos, inv)
+
+
 def test_non_finite_values_stay_in_their_pair():
     q = torch.ones(1, 2, 1, 64, dtype=torch.float16)
     q[0, 0, 0, 3] = math.inf
