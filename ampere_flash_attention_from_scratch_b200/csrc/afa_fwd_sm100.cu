@@ -284,7 +284,7 @@ const char* afa_strerror(int code) {
     case AFA_ERR_LAUNCH: return "kernel launch failed";
     case AFA_ERR_DEVICE_TIMEOUT: return "a device-side bounded wait ran out; the kernel aborted";
     case AFA_ERR_TOO_LARGE: return "problem size exceeds 32-bit work-item / coordinate indexing";
-    case AFA_ERR_SCRATCH_LIMIT: return "afa_fwd_sm100_noalloc: the call needs more scratch memory than the library's static array (AFA_NOALLOC_SCRATCH_BYTES) holds";
+    case AFA_ERR_SCRATCH_LIMIT: return "the call needs more scratch memory than it may use (afa_fwd_sm100_noalloc: AFA_NOALLOC_SCRATCH_BYTES; afa_cache4_fwd_sm100: workspace_bytes)";
     default: return "unknown error";
   }
 }

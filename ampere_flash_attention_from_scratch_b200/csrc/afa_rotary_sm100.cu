@@ -12,7 +12,12 @@
 // all, against 3 fp32 operations.  The angles are shared by all heads of a
 // token, so a CTA forms them once for its tokens (rot_dim / 2 of them a token),
 // keeps cosine and sine in shared memory and turns every query and key head of
-// those tokens in the same pass: one launch for q and k.
+// those tokens in the same pass: one launch for q and k.  32 bytes an access
+// where the layout allows it, two or four rows of a thread in flight.
+// Measured: [2, 8190, 32 + 32, 64] fp16, three axes, neighbouring pairs 46 us =
+// 5.9 TB/s (89 % of the measured copy bandwidth; 6.5 TB/s inside the kernel);
+// [4, 4099, 32 + 8, 128] bf16 forward and backward 121 us = 5.6 TB/s in two
+// launches; 64 tokens [32 + 8, 128] 4 us, the launch itself.
 #include "ops_common.cuh"
 
 namespace {
