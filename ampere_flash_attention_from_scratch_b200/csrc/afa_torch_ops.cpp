@@ -64,8 +64,11 @@ at::Tensor fresh_tensor(at::IntArrayRef shape, at::ScalarType type, const at::De
   return at::Tensor(at::detail::empty_cuda(shape, type, dev, std::nullopt));
 }
 
-// A tensor of the caller's has been written: autograd notices if it had saved it.
-void written(const at::Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+// A tensor of the caller's has been written: autograd notices if it had saved
+// it.  (Tensors made in inference mode have no version, and are never saved.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 
 // `out` if given (checked against `like`), else a new contiguous tensor.
 at::Tensor output_like(const std::optional<at::Tensor>& out, const at::Tensor& like, const char* name) {

@@ -355,7 +355,7 @@ def test_negative_steps_are_taken_as_written():
 
 
 # --- lengths and pages that are wrong --------------------------------------------------------------------
-@pytest.mark.parametrize("entry", ["write", "read", "attend"])
+@pytest.mark.parametrize("entry", ["write", "read", "attend", "attend many"])
 @pytest.mark.parametrize("fault", ["page low", "page high", "length high", "length low", "new high", "new low"])
 def test_bad_tables_and_lengths_are_reported(entry, fault):
     table, lens, new = ints([[0, 1], [2, 3]]), ints([20, 30]), ints([2, 2])
@@ -379,8 +379,9 @@ def test_bad_tables_and_lengths_are_reported(entry, fault):
         fa.cache4_write(x, x, cache, table, lens, new)
     elif entry == "read":
         fa.cache4_read(cache, table, lens, 2, torch.float16, new)
-    else:
-        fa.forward_cache4(x, cache, table, lens, new_lens=new)
+    else:  # 2 or 128 query rows
+        q = x if entry == "attend" else x.expand(2, 2, 64, 64)
+        fa.forward_cache4(q, cache, table, lens, new_lens=new)
     torch.cuda.synchronize()
     want = "page_table" if fault.startswith("page") else "kv_lens"
     with pytest.raises(RuntimeError, match=f"earlier launch on cuda:0.*{want}"):
@@ -485,7 +486,8 @@ def test_wait_that_runs_out_is_reported():
 
 
 # --- streams, graphs, several calls ----------------------------------------------------------------------
-def test_captured_steps_follow_their_inputs():
+@pytest.mark.parametrize("group", [4, 80])
+def test_captured_steps_follow_their_inputs(group):
     # a decode step (write, attend) captured once and replayed as the sequences grow; two graphs side by side
     d, page, heads = 128, 16, 2
     graphs = []
@@ -493,7 +495,7 @@ def test_captured_steps_follow_their_inputs():
         table = torch.arange(8, dtype=torch.int32).view(2, 4).cuda()
         cache = torch.zeros(8, heads, 2, page, 72, dtype=torch.uint8, device="cuda")
         k, v = (torch.zeros(2, 1, heads, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
-        q = torch.zeros(2, 1, 4 * heads, d, dtype=torch.bfloat16, device="cuda")
+        q = torch.zeros(2, 1, group * heads, d, dtype=torch.bfloat16, device="cuda")
         lens = ints([1, 1]).cuda()
         stream = torch.cuda.Stream()
         stream.wait_stream(torch.cuda.current_stream())
@@ -523,12 +525,15 @@ def test_captured_steps_follow_their_inputs():
     fa.check_status(0)
 
 
-def test_calls_at_once_on_two_streams_agree_with_one():
+@pytest.mark.parametrize("n", [3, 40])
+def test_calls_at_once_on_two_streams_agree_with_one(n):
     lens = [900, 1300, 5, 0]
     cache, table = filled(lens, 2, 128, 32, torch.float16, seed=4)
     cache, table, lens = cache.cuda(), table.cuda(), ints(lens).cuda()
-    qs = [torch.randn(4, 3, 8, 128, generator=torch.Generator().manual_seed(i)).half().cuda() for i in range(2)]
+    qs = [torch.randn(4, n, 8, 128, generator=torch.Generator().manual_seed(i)).half().cuda() for i in range(2)]
     want = [fa.forward_cache4(q, cache, table, lens, None, True, None, True) for q in qs]
+    dense = torch.randn(1, 512, 4, 128, generator=torch.Generator().manual_seed(5)).half().cuda()
+    want_dense, _ = fa.forward_ext(dense, dense, dense)
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in qs]
     for _ in range(20):
@@ -536,7 +541,9 @@ def test_calls_at_once_on_two_streams_agree_with_one():
         for q, s in zip(qs, streams):
             with torch.cuda.stream(s):
                 got.append(fa.forward_cache4(q, cache, table, lens, None, True, None, True))
+        between, _ = fa.forward_ext(dense, dense, dense)  # the dense kernel beside them
         torch.cuda.synchronize()
+        assert torch.equal(between, want_dense)
         for a, b in zip(want, got):
             assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
         del got
@@ -591,6 +598,38 @@ def test_far_pages_pass_32_bit_offsets():
                                                  fa.cache4_read(small, near, lens, 200, torch.float16)))
     check_attention(q, small.cpu(), near.cpu(), [200, 200], False, got=(o, lse))
     fa.check_status(0)
+
+
+@pytest.mark.parametrize("case", [([1500, 700], 700, 8, 2, 128, 64, torch.bfloat16), ([900], 900, 4, 4, 64, 16, torch.float16)],
+                         ids=lambda c: f"n{c[1]}-d{c[4]}")
+def test_prompt_sized_chunks(case):
+    # hundreds of new tokens at once, causal; the oracle's formulas on the GPU
+    lens, n, H, HK, d, page, dtype = case
+    new = [n, n - 300][: len(lens)]
+    cache, table = filled(lens, HK, d, page, dtype, seed=12)
+    q = torch.randn(len(lens), n, H, d, generator=torch.Generator().manual_seed(2)).to(dtype)
+    o, lse = fa.forward_cache4(q.cuda(), cache.cuda(), table.cuda(), ints(lens).cuda(), None, True, None, True, ints(new).cuda())
+    fa.check_status(0)
+    for b, length in enumerate(lens):
+        m = new[b]
+        assert not o[b, m:].any() and torch.all(lse[b, :, m:] == -math.inf)
+        part = []
+        for r in oc.sequence_rows(cache, table, b, length):
+            c, s, mn = oc.unpack_rows(r, dtype)
+            part += [(c * s.repeat_interleave(64, -1)).cuda(), mn.repeat_interleave(64, -1).cuda()]
+        kc, km, vc, vm = [x.transpose(0, 1).repeat_interleave(H // HK, 0) for x in part]  # [H, T, d]
+        x = q[b, :m].cuda().double().transpose(0, 1)
+        sees = torch.arange(length, device="cuda") <= length - m + torch.arange(m, device="cuda")[:, None]
+        score = (x @ (kc + km).transpose(1, 2) / math.sqrt(d)).masked_fill(~sees, -math.inf)
+        reach = (x.abs() @ (kc + km.abs()).transpose(1, 2) / math.sqrt(d)).masked_fill(~sees, 0).amax(-1)
+        p = torch.softmax(score, -1)
+        want, weight = p @ (vc + vm), p @ (vc + vm.abs())
+        err = (o[b, :m].double().transpose(0, 1) - want).abs()
+        eps = torch.finfo(dtype).eps
+        tol = want.abs() * eps / 2 + (2.0 ** -11 + 2.0 ** -18 * reach[..., None] + 2.0 ** -15) * weight + TINY[dtype]
+        assert torch.all(err <= tol), f"largest error over tolerance {(err / tol).max().item():.3f}"
+        want_lse = torch.logsumexp(score, -1)
+        assert torch.all((lse[b, :, :m].double() - want_lse).abs() <= 2.0 ** -19 * reach + 2.0 ** -15 + 2.0 ** -22 * want_lse.abs())
 
 
 # --- together --------------------------------------------------------------------------------------------
