@@ -9,6 +9,7 @@ namespace afa100 {
 
 constexpr int kUnit = 128;        // tokens of a unit of work
 constexpr int kItemUnits = 4;     // units an item is charged beside its tokens'
+constexpr int kWholeTokens = 512; // items that cannot be longer are not split, if there is a CTA for each
 constexpr float kRescale = 8.0f;  // log2 units a score may pass the reference maximum by
 constexpr float kHeadroom = 7.0f; // log2 of p s' at the reference maximum and the largest step
 
@@ -26,6 +27,8 @@ struct FwdParams4 {
   int32_t page_shift;
   uint32_t page_stride;
   int32_t causal;
+  int32_t unit_tokens;  // kUnit, or kWholeTokens where items are not split
+  int32_t item_units;   // kItemUnits, or 0
   float scale_log2;
   uint64_t timeout_ns;  // of a wait (the kernel for many rows; the other one waits for nothing)
   uint32_t test_flags;  // AFA_TEST_PRODUCER_IDLE
@@ -61,10 +64,10 @@ __device__ __forceinline__ int tokens_of(const FwdParams4& p, int b) {
   }
   return kv;
 }
-// Units of an item: kItemUnits that stand for what starting and ending an item
+// Units of an item: item_units that stand for what starting and ending an item
 // costs, then those of its tokens (one at least).
-__device__ __forceinline__ int units_of(int tokens) {
-  return kItemUnits + (tokens <= kUnit ? 1 : (tokens + kUnit - 1) / kUnit);
+__device__ __forceinline__ int units_of(const FwdParams4& p, int tokens) {
+  return p.item_units + (tokens <= p.unit_tokens ? 1 : (tokens + kUnit - 1) / kUnit);
 }
 
 struct Division {
@@ -87,7 +90,7 @@ __device__ __forceinline__ Division divide(const FwdParams4& p, int per, int gri
   int mine = 0;
   for (int i = 0; i < per; ++i) {
     const int b = lane * per + i;
-    if (b < p.c.batch) mine += units_of(tokens_of(p, b));
+    if (b < p.c.batch) mine += units_of(p, tokens_of(p, b));
   }
   mine *= p.c.n_kv_heads * p.row_tiles;
   int upto = mine;
@@ -124,7 +127,7 @@ __device__ __forceinline__ Item find_item(const FwdParams4& p, int per, int befo
   it.b = owner * per;
   for (;;) {
     it.tokens = tokens_of(p, it.b);
-    it.units = units_of(it.tokens);
+    it.units = units_of(p, it.tokens);
     const int here = it.units * items;
     if (left < here || it.b + 1 >= p.c.batch) break;
     left -= here;
@@ -142,10 +145,10 @@ struct Walk {
   int left;      // units of the CTA from this piece on
   int unit_end;  // end of the piece within the item
   int tok, tok_end;
-  __device__ __forceinline__ void open(int offset) {
+  __device__ __forceinline__ void open(const FwdParams4& p, int offset) {
     unit_end = it.unit + left < it.units ? it.unit + left : it.units;
-    tok = max(it.unit - kItemUnits, 0) * kUnit + offset;
-    tok_end = min(it.tokens, max(unit_end - kItemUnits, 0) * kUnit);
+    tok = max(it.unit - p.item_units, 0) * p.unit_tokens + offset;
+    tok_end = min(it.tokens, max(unit_end - p.item_units, 0) * p.unit_tokens);
   }
   // To the next piece; false at the end of the CTA's units.
   __device__ __forceinline__ bool next(const FwdParams4& p, int offset) {
@@ -157,9 +160,9 @@ struct Walk {
       it.which = 0;
       ++it.b;
       it.tokens = tokens_of(p, it.b);
-      it.units = units_of(it.tokens);
+      it.units = units_of(p, it.tokens);
     }
-    open(offset);
+    open(p, offset);
     return true;
   }
 };

@@ -145,12 +145,12 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 || kD == 64 ? 3 : 2) cache4
     if (cta >= div.ctas) return;
     w.it = find_item(p, per, before_lane, div.first(cta));
     w.left = div.first(cta + 1) - div.first(cta);
-    w.open(warp * kStep);
+    w.open(p, warp * kStep);
   }
   // Past pieces that are only the cost of an item whose tokens another CTA has; false at the end.
   auto skip_empty = [&](Walk& walk) {
     bool go = true;
-    while (go && walk.unit_end <= kItemUnits) go = walk.next(p, warp * kStep);
+    while (go && walk.unit_end <= p.item_units) go = walk.next(p, warp * kStep);
     return go;
   };
 
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 || kD == 64 ? 3 : 2) cache4
   for (;;) {
     const Item it = w.it;
     const int head = it.which / p.row_tiles, tile = it.which - head * p.row_tiles;
-    const bool starts = it.unit <= kItemUnits, whole = starts && w.unit_end == it.units;
+    const bool starts = it.unit <= p.item_units, whole = starts && w.unit_end == it.units;
     const int fresh = p.c.new_lens != nullptr ? p.c.new_lens[it.b] : p.seq_len;
 
     // --- queries: rows on the N side, their channels in the order the codes come ------------------------
@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(128) cache4_join_kernel(const FwdParams4 p) {
   if (mine) {
     const int u = div.first(cta);
     const Item it = find_item(p, per, before_lane, u);
-    const int begin = u - it.unit + kItemUnits, end = u - it.unit + it.units;  // of the tokens' units
+    const int begin = u - it.unit + p.item_units, end = u - it.unit + it.units;  // of the tokens' units
     mine = u > begin && div.first(cta - 1) <= begin;
     head = it.which / p.row_tiles;
     tile = it.which - head * p.row_tiles;
@@ -714,7 +714,7 @@ template <int kD, bool kBF16, int kNT>
 cudaError_t join4(const FwdParams4& p, unsigned grid, cudaStream_t s) {
   using L = FwdLayout4<kD, kNT>;
   const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || grid == 1) return e;
+  if (e != cudaSuccess || grid == 1 || p.item_units == 0) return e;  // one CTA or no split item: no shares
   cudaLaunchAttribute overlap{};
   overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   overlap.val.programmaticStreamSerializationAllowed = 1;
@@ -764,9 +764,9 @@ const Kernel4 kKernels4[2][2][3] = {{AFA_ROWS4(64, false), AFA_ROWS4(64, true)},
 std::mutex g_mu4;
 int g_ctas_per_sm[kOpsMaxDevices][2][2][3] = {};
 
-// Kernel, grid and row blocks of a call.
+// Kernel, grid and row blocks of a call, and whether its items are not split.
 int plan4(const AfaCache4* c, int32_t seq_len, int32_t n_heads, const Kernel4** kernel, int32_t* grid,
-          int32_t* row_tiles) {
+          int32_t* row_tiles, bool* whole) {
   int rc = ops_check_cache(c);
   if (rc != AFA_OK) return rc;
   if (seq_len <= 0 || n_heads <= 0 || n_heads % c->n_kv_heads != 0) return AFA_ERR_INVALID_ARGUMENT;
@@ -799,8 +799,12 @@ int plan4(const AfaCache4* c, int32_t seq_len, int32_t n_heads, const Kernel4** 
     }
     *grid = sms * per_sm;
   }
+  // Short sequences, few of them: one CTA an item.  The host then launches one kernel instead of two (7.5 us a call
+  // instead of 9.8), and on the device 32/8 heads of 128 in bf16 take, split -> whole, us in a row: 32 sequences of
+  // 500 tokens 16.4 -> 12.3, 1 of 500 10.2 -> 10.2, 1 of 1000 10.3 -> 12.7.  The tcgen05 kernel keeps the split.
+  *whole = ni < 2 && int64_t{c->max_pages} * c->page_size <= kWholeTokens && items * c->batch <= *grid;
   // no more CTAs than units at the sequences' largest possible lengths
-  const int64_t most = units * items * c->batch;
+  const int64_t most = *whole ? items * c->batch : units * items * c->batch;
   if (most < *grid) *grid = static_cast<int32_t>(most);
   *kernel = &k;
   *row_tiles = static_cast<int32_t>(tiles);
@@ -814,7 +818,8 @@ extern "C" {
 int64_t afa_cache4_fwd_workspace(const AfaCache4* cache, int32_t seq_len, int32_t n_heads) {
   const Kernel4* k = nullptr;
   int32_t grid = 0, tiles = 0;
-  const int rc = plan4(cache, seq_len, n_heads, &k, &grid, &tiles);
+  bool whole = false;
+  const int rc = plan4(cache, seq_len, n_heads, &k, &grid, &tiles, &whole);
   if (rc != AFA_OK) return -static_cast<int64_t>(rc);
   return int64_t{2} * grid * k->share_floats * static_cast<int64_t>(sizeof(float));
 }
@@ -832,7 +837,8 @@ int afa_cache4_fwd_sm100(const AfaCache4* cache, const AfaCache4FwdArgs* a, void
     return AFA_ERR_MISALIGNED;
   const Kernel4* k = nullptr;
   int32_t grid = 0, tiles = 0;
-  rc = plan4(cache, a->seq_len, a->n_heads, &k, &grid, &tiles);
+  bool whole = false;
+  rc = plan4(cache, a->seq_len, a->n_heads, &k, &grid, &tiles, &whole);
   if (rc != AFA_OK) return rc;
   if (a->workspace_bytes < int64_t{2} * grid * k->share_floats * static_cast<int64_t>(sizeof(float)))
     return AFA_ERR_SCRATCH_LIMIT;
@@ -854,6 +860,8 @@ int afa_cache4_fwd_sm100(const AfaCache4* cache, const AfaCache4FwdArgs* a, void
   p.row_tiles = tiles;
   p.page_shift = ops_log2(cache->page_size);
   p.page_stride = static_cast<uint32_t>(cache->page_stride);
+  p.unit_tokens = whole ? kWholeTokens : kUnit;
+  p.item_units = whole ? 0 : kItemUnits;
   p.causal = a->causal;
   p.timeout_ns = a->timeout_ns != 0 ? a->timeout_ns : 4000000000ull;
   p.test_flags = a->test_flags;

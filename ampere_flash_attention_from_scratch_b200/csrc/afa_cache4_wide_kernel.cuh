@@ -382,9 +382,9 @@ __device__ __forceinline__ void wide_softmax(const FwdParams4& p, Walk w, char* 
   bool ok = true;
   do {
     const Item it = w.it;
-    if (w.unit_end <= kItemUnits) continue;  // only the cost of an item that another CTA works on
+    if (w.unit_end <= p.item_units) continue;  // only the cost of an item that another CTA works on
     const int head = it.which / p.row_tiles, tile = it.which - head * p.row_tiles;
-    const bool starts = it.unit <= kItemUnits, whole = starts && w.unit_end == it.units;
+    const bool starts = it.unit <= p.item_units, whole = starts && w.unit_end == it.units;
     const int fresh = fresh_of(p, it.b);
     const int stop = min(w.tok_end, wide_reach(p, it, fresh));
     const int tile_rows = min(128, p.rows - tile * 128);
@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(WideLayout<kD>::kThreads, 2) cache4_wide_kerne
     if (cta >= div.ctas) return;
     w.it = find_item(p, per, before_lane, div.first(cta));
     w.left = div.first(cta + 1) - div.first(cta);
-    w.open(0);
+    w.open(p, 0);
   }
   if (warp == 0) {
     if (lane == 0) {

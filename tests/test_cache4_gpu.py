@@ -285,6 +285,19 @@ def test_random_shapes(d, dtype):
         check_attention(q, cache, table, lens, bool(r(0, 1)), new)
 
 
+@pytest.mark.parametrize("n", [1, 6, 30])
+def test_tables_wider_than_the_sequences(n):
+    # the same sequences by tables of 512 tokens' capacity and more: items in one piece and in several
+    lens, page = [512, 0, 301, 1, 128], 16
+    cache, table = filled(lens, 3, 128, page, torch.bfloat16, seed=n)
+    q = torch.randn(5, n, 6, 128, generator=torch.Generator().manual_seed(n)).bfloat16()
+    assert table.shape[1] >= 32
+    for width in (32, 33, 64, 200):
+        wide = torch.full((5, width), -1, dtype=torch.int32)
+        wide[:, :32] = table[:, :32]
+        check_attention(q, cache, wide, lens, True)
+
+
 @pytest.mark.parametrize("k_scale,v_scale,q_scale", [(8.0, 1.0, 3.0), (1e-3, 1e-4, 1.0), (1.0, 200.0, 30.0), (30.0, 1.0, 1e-3)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_ranges(dtype, k_scale, v_scale, q_scale):
