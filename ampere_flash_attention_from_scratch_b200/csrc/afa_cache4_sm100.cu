@@ -13,9 +13,9 @@
 // minimum and maximum travel together as one packed pair through two shuffles.  A CTA
 // takes a tile of tokens of one sequence times (head, keys or values), tokens
 // fastest, so that the rows it writes are neighbours in a page.
-// Measured: reading back 131072 tokens [8, 128] bf16 114 us = 6.0 TB/s (92 % of
+// Measured: reading back 131072 tokens [8, 128] bf16 109 us = 6.3 TB/s (96 % of
 // the measured copy bandwidth).  Eight prompts of 4096 down to 2304 tokens
-// [8, 128] fp16, written and read back: 70 us = 4.2 TB/s (65 %); the reader is
+// [8, 128] fp16, written and read back: 66 us = 4.5 TB/s (69 %); the reader is
 // at the bandwidth there too, the writer at its arithmetic (about 17
 // instructions a value, 69 % of the issue slots), so one row a lane (83 us) and
 // four (76 us) are slower than two.
@@ -255,6 +255,7 @@ template <int kD, bool kBF16, bool kLong>
 __global__ void __launch_bounds__(kThreads) cache4_write_kernel(const Cache4Params p) {
   using T = Tile<kD>;
   const Place<kD, kLong> at(p);
+  after_previous();
   const NewRows fresh = new_rows(p.c, at.b, p.seq_len);
   if (at.token0 >= fresh.count) return;
   const int lane = threadIdx.x % T::kLanes;
@@ -318,6 +319,7 @@ template <int kD, bool kBF16, bool kLong>
 __global__ void __launch_bounds__(kThreads) cache4_read_kernel(const Cache4Params p) {
   using T = Tile<kD>;
   const Place<kD, kLong> at(p);
+  after_previous();
   const NewRows fresh = new_rows(p.c, at.b, p.seq_len);
   const int lane = threadIdx.x % T::kLanes;
   uint2 word[kUnroll];
@@ -392,11 +394,8 @@ int cache4_move(const AfaCache4* c, const void* k, const void* v, const int64_t*
   const auto s = static_cast<cudaStream_t>(stream);
   const bool bf = c->dtype == AFA_DTYPE_BF16;
   const bool one_side = (1 << p.tile_shift) == tile;
-#define AFA_MOVE_AS(D, BF, LONG)                             \
-  if (kWrite)                                                \
-    cache4_write_kernel<D, BF, LONG><<<g, kThreads, 0, s>>>(p); \
-  else                                                       \
-    cache4_read_kernel<D, BF, LONG><<<g, kThreads, 0, s>>>(p)
+#define AFA_MOVE_AS(D, BF, LONG) \
+  ops_launch(kWrite ? cache4_write_kernel<D, BF, LONG> : cache4_read_kernel<D, BF, LONG>, dim3(g), kThreads, 0, s, p)
 #define AFA_MOVE(D, BF)          \
   if (one_side) {                \
     AFA_MOVE_AS(D, BF, true);    \

@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(WideLayout<kD>::kThreads, 2) cache4_wide_kerne
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kOffAbort);
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take the SMs as they fall free
+  after_previous();  // and the join may take the SMs as they fall free
   Walk w;
   {
     const int per = (p.c.batch + 31) / 32;

@@ -14,10 +14,10 @@
 // keeps cosine and sine in shared memory and turns every query and key head of
 // those tokens in the same pass: one launch for q and k.  32 bytes an access
 // where the layout allows it, two or four rows of a thread in flight.
-// Measured: [2, 8190, 32 + 32, 64] fp16, three axes, neighbouring pairs 46 us =
+// Measured: [2, 8190, 32 + 32, 64] fp16, three axes, neighbouring pairs 44 us =
 // 5.9 TB/s (89 % of the measured copy bandwidth; 6.5 TB/s inside the kernel);
-// [4, 4099, 32 + 8, 128] bf16 forward and backward 121 us = 5.6 TB/s in two
-// launches; 64 tokens [32 + 8, 128] 4 us, the launch itself.
+// [4, 4099, 32 + 8, 128] bf16 forward and backward 117 us = 5.8 TB/s in two
+// launches; 64 tokens [32 + 8, 128] 2.7 us, the launch itself.
 #include "ops_common.cuh"
 
 namespace {
@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
   const int token0 = blockIdx.x * p.tokens;
   const int n_tok = min(p.tokens, p.n_tokens - token0);
   const int blocks = p.half / kPairs;
+  after_previous();
   if (threadIdx.x < 2 * n_tok) {
     const int t = threadIdx.x >> 1, w = threadIdx.x & 1;
     const int b = (token0 + t) / p.seq_len, n = (token0 + t) - b * p.seq_len;
@@ -171,11 +172,11 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
 template <bool kBF16>
 void launch_rotary(Layout layout, unsigned grid, size_t smem, cudaStream_t s, const RotaryParams& p) {
   if (layout == kNeighbours)
-    rotary_kernel<kBF16, kNeighbours><<<grid, kThreads, smem, s>>>(p);
+    ops_launch(rotary_kernel<kBF16, kNeighbours>, dim3(grid), kThreads, smem, s, p);
   else if (layout == kHalvesWide)
-    rotary_kernel<kBF16, kHalvesWide><<<grid, kThreads, smem, s>>>(p);
+    ops_launch(rotary_kernel<kBF16, kHalvesWide>, dim3(grid), kThreads, smem, s, p);
   else
-    rotary_kernel<kBF16, kHalvesNarrow><<<grid, kThreads, smem, s>>>(p);
+    ops_launch(rotary_kernel<kBF16, kHalvesNarrow>, dim3(grid), kThreads, smem, s, p);
 }
 
 }  // namespace

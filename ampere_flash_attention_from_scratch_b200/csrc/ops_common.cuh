@@ -47,6 +47,35 @@ inline int ops_launched() {
   return AFA_OK;
 }
 
+// A launch whose CTAs may take their places while the stream's kernel before
+// it ends; the kernel calls after_previous() before it touches global memory.
+// Calls in a row, plain -> so: rotary of 64 tokens 4.1 -> 2.7 us, a token
+// written to 128 sequences and read back 8.2 -> 5.2, attention over 500 tokens
+// 10.3 -> 8.0; the large cases lose 2 to 3 us; the host's side is no longer.
+template <class... P, class... A>
+inline cudaError_t ops_launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s,
+                              const A&... args) {
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &overlap;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Waits until the stream's earlier kernels have ended and their writes are
+// seen, then lets the next one's CTAs in: in this order, so that whatever that
+// one reads before its own wait is not written by kernels before this one.
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 inline bool ops_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0u; }
 
 // Strides (batch, seq, head) of a 16-bit tensor whose rows are moved 16 bytes

@@ -645,6 +645,46 @@ def test_prompt_sized_chunks(case):
         assert torch.all((lse[b, :, :m].double() - want_lse).abs() <= 2.0 ** -19 * reach + 2.0 ** -15 + 2.0 ** -22 * want_lse.abs())
 
 
+@pytest.mark.parametrize("capacity,n,HK", [(512, 1, 2), (2048, 2, 2), (4096, 24, 1)])
+def test_calls_in_a_row_see_each_other(capacity, n, HK):
+    # each call's inputs are the outputs of the one before, and the next one starts while that ends: the same as with
+    # the device idle in between; narrow in one launch, in two, and the kernel for many rows
+    d, page, H, B = 64, 16, 4 * HK, 3
+    g = torch.Generator().manual_seed(capacity)
+    first = torch.randn(B, n, H, d, generator=g).half().cuda()
+    old = torch.randn(B, capacity, HK, d, generator=g).half().cuda()
+    table = torch.randperm(B * capacity // page, generator=g).view(B, -1).int().cuda()
+    inv = (10000.0 ** (-torch.arange(32, dtype=torch.float64) / 32)).float().cuda()
+
+    def run(idle):
+        wait = torch.cuda.synchronize if idle else lambda: None
+        cache = noise_cache(B * capacity // page, HK, page, d).cuda()
+        fa.cache4_write(old, old, cache, table, ints([capacity] * B).cuda())
+        lens = ints([capacity - 60 * n, 5, capacity // 2]).cuda()
+        q, seen = first, []
+        for _ in range(50):
+            lens.add_(n)
+            wait()
+            pos = (lens[:, None] - n + torch.arange(n, device="cuda")).unsqueeze(0)
+            q, k = fa.rotary(q, q[:, :, :HK], pos, inv, [32])
+            wait()
+            fa.cache4_write(k, q[:, :, HK:2 * HK], cache, table, lens)
+            wait()
+            o, _ = fa.forward_cache4(q, cache, table, lens, None, True)
+            wait()
+            back, _ = fa.cache4_read(cache, table, lens, n, torch.float16)
+            wait()
+            q = (o + back.repeat_interleave(4, 2)).clamp_(-4, 4)
+            seen.append(q)
+        torch.cuda.synchronize()
+        return torch.stack(seen), cache
+
+    want, got = run(True), run(False)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    assert torch.isfinite(got[0]).all() and got[0][-1].any()
+    fa.check_status(0)
+
+
 # --- together --------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_prompt_then_tokens(dtype):
