@@ -820,7 +820,8 @@ int afa_cache4_fwd_sm100(const AfaCache4* cache, const AfaCache4FwdArgs* a, void
   int rc = ops_check_cache(cache);
   if (rc != AFA_OK) return rc;
   if (a == nullptr || a->q == nullptr || a->o == nullptr || a->workspace == nullptr ||
-      (a->causal != 0 && a->causal != 1) || a->seq_len <= 0 || a->n_heads <= 0)
+      (a->causal != 0 && a->causal != 1) || a->seq_len <= 0 || a->n_heads <= 0 ||
+      !(a->scale < 1e38f))  // NaN, or beyond fp32 times log2(e)
     return AFA_ERR_INVALID_ARGUMENT;
   if (!ops_aligned16(a->q) || !ops_aligned16(a->o) || !ops_aligned16(a->workspace) ||
       (reinterpret_cast<uintptr_t>(a->lse) & 3u) != 0u ||

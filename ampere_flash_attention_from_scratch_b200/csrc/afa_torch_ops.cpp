@@ -432,6 +432,7 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> forward_cache4(
   if (softmax_scale.has_value()) {
     scale = softmax_scale.value();
     TORCH_CHECK(scale > 0.0, "softmax_scale must be positive");
+    TORCH_CHECK(static_cast<float>(scale) > 0.0f && scale < 1e38, "softmax_scale ", scale, " is not one of fp32's range");
   }
   const at::Tensor o = output_like(o_, q, "o");
   const int32_t n = static_cast<int32_t>(q.size(1)), heads = static_cast<int32_t>(q.size(2));

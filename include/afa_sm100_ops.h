@@ -143,7 +143,7 @@ typedef struct AfaCache4FwdArgs {
   int32_t seq_len;
   int32_t n_heads;
   int32_t causal;
-  float scale; /* <= 0 selects 1/sqrt(head_dim) */
+  float scale; /* <= 0 selects 1/sqrt(head_dim); below 1e38, not NaN */
   uint64_t timeout_ns; /* bound of every device-side wait; 0 selects the default (4 s) */
   uint32_t test_flags; /* 0 in normal use; AFA_TEST_PRODUCER_IDLE: in calls of more than 64 query rows a
                           key/value head nothing is loaded, and the bounded waits run out */

@@ -456,7 +456,8 @@ def test_refusals():
         with pytest.raises(RuntimeError, match=match):
             r(**over)
     for over, match in [(dict(q=x[:, :, :1]), "multiple of"), (dict(q=x.float()), "Only fp16"), (dict(q=x[..., :32].contiguous()), "differ"),
-                        (dict(softmax_scale=0.0), "softmax_scale"), (dict(o=x[:1]), "same shape"), (dict(o=x.bfloat16()), "dtype")]:
+                        (dict(softmax_scale=0.0), "softmax_scale"), (dict(softmax_scale=1e-60), "fp32's range"),
+                        (dict(softmax_scale=math.inf), "fp32's range"), (dict(softmax_scale=math.nan), "positive"), (dict(o=x[:1]), "same shape"), (dict(o=x.bfloat16()), "dtype")]:
         with pytest.raises(RuntimeError, match=match):
             a(**over)
     fa.check_status(0)
@@ -535,6 +536,53 @@ def test_captured_steps_follow_their_inputs(group):
         if step % 13 == 0:
             for _, _, k, v, q, lens, cache, table, o, lse in graphs:
                 check_attention(q.cpu(), cache.cpu(), table.cpu(), lens.tolist(), False, got=(o, lse))
+    fa.check_status(0)
+
+
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_capture_behind_copies_and_joined_streams(n):
+    # calls whose predecessors in a graph are a copy, a fill, or the ends of two streams, and a call on a side stream
+    d, page, B, HK = 128, 16, 2, 2
+    g = torch.Generator().manual_seed(n)
+    cache, table = filled([400, 70], HK, d, page, torch.bfloat16, seed=n)
+    cache, table, lens = cache.cuda(), table.cuda(), ints([400, 70]).cuda()
+    fresh = [torch.randn(B, n, 4 * HK, d, generator=g).bfloat16().cuda() for _ in range(3)]
+    inv = (10000.0 ** (-torch.arange(64, dtype=torch.float64) / 64)).float().cuda()
+    pos = torch.zeros(1, B, n, dtype=torch.int32, device="cuda")
+    x, q, o = (torch.zeros_like(fresh[0]) for _ in range(3))
+    fill = torch.ones_like(x)
+
+    def step(main, side):
+        q.copy_(x)
+        pos.fill_(7)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            turned, _ = fa.rotary(q, None, pos, inv)
+            k = turned[:, :, :HK]
+            fa.cache4_write(k, k, cache, table, lens)
+        fill.zero_()
+        main.wait_stream(side)
+        fa.forward_cache4(turned, cache, table, lens, o, True)
+        fill.add_(o)
+        back, _ = fa.cache4_read(cache, table, lens, n, torch.bfloat16)
+        return turned, back
+
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(main):
+        step(main, side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=main):
+            turned, back = step(main, side)
+        for f in fresh:
+            x.copy_(f)
+            graph.replay()
+            torch.cuda.synchronize()
+            want, _ = fa.rotary(f, None, pos, inv)
+            assert torch.equal(turned, want) and torch.equal(fill, o)
+            check_attention(want.cpu(), cache.cpu(), table.cpu(), [400, 70], True,
+                            got=(o, fa.forward_cache4(want, cache, table, lens, None, True, None, True)[1]))
+            assert torch.equal(back, fa.cache4_read(cache, table, lens, n, torch.bfloat16)[0])
     fa.check_status(0)
 
 

@@ -202,6 +202,8 @@ def fwd_args(**over):
     (dict(n_heads=0), _abi.AFA_ERR_INVALID_ARGUMENT),
     (dict(n_heads=6), _abi.AFA_ERR_INVALID_ARGUMENT),  # not a multiple of 4 key/value heads
     (dict(causal=2), _abi.AFA_ERR_INVALID_ARGUMENT),
+    (dict(scale=float("nan")), _abi.AFA_ERR_INVALID_ARGUMENT),
+    (dict(scale=3e38), _abi.AFA_ERR_INVALID_ARGUMENT),
     (dict(q=0x100008), _abi.AFA_ERR_MISALIGNED),
     (dict(workspace=0x100008), _abi.AFA_ERR_MISALIGNED),
     (dict(lse=0x100002), _abi.AFA_ERR_MISALIGNED),
