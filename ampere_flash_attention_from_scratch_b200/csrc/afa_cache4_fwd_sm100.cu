@@ -27,12 +27,12 @@
 // from HBM alike.  Hence tokens on the M side of mma.m16n8k16 (16 tokens x 8 query
 // rows): one row and eight cost the same, and no lane idles on a row block padded
 // to 128, for which the codes would also have to be spread in shared memory.
-// Measured: [8 x 131072 tokens, 32/8 heads, 128] bf16 250 us = 4.8 TB/s (74 % of the
+// Measured: [8 x 131072 tokens, 32/8 heads, 128] bf16 240 us = 5.0 TB/s (77 % of the
 // measured copy bandwidth; 203 us with the arithmetic left out); [32 x 256..8192,
-// 32/8, 128] bf16 43 us = 3.6 TB/s; [16 x 250..4001, 32/32, 64] fp16 33 us = 2.4
+// 32/8, 128] bf16 41 us = 3.8 TB/s; [16 x 250..4001, 32/32, 64] fp16 31 us = 2.6
 // TB/s (one of eight columns used, half the channels for the same softmax).
-// 500 tokens: 7 us on the device, the work's division, two dependent loads and
-// the join.  4 CTAs an SM instead of 3 and 4 steps in the ring instead of 3: equal
+// 500 tokens: 8 us on the device, the work's division, two dependent loads and
+// four steps of a warp.  4 CTAs an SM instead of 3 and 4 steps in the ring instead of 3: equal
 // to 3 % slower.
 //
 // Work.  The (sequence, key/value head, row block) items are cut into units of
