@@ -586,6 +586,28 @@ def test_capture_behind_copies_and_joined_streams(n):
     fa.check_status(0)
 
 
+def test_inference_mode():
+    # tensors without a version counter, as inputs, caches and given outputs
+    table, lens = ints([[0, 1]]).cuda(), ints([20]).cuda()
+    x = torch.randn(1, 20, 2, 64, generator=torch.Generator().manual_seed(1)).half().cuda()
+    inv, pos = torch.ones(32, device="cuda"), torch.arange(20, device="cuda").view(1, 1, 20)
+
+    def run():
+        cache = fa.cache4_empty(2, 2, 16, 64)
+        q, k = fa.rotary(x, x, pos, inv, q_out=torch.empty_like(x), k_out=torch.empty_like(x))
+        fa.cache4_write(k, x, cache, table, lens)
+        back = [torch.empty_like(x) for _ in range(2)]
+        fa.cache4_read(cache, table, lens, 20, torch.float16, None, *back)
+        o = torch.empty_like(x)
+        fa.forward_cache4(q, cache, table, lens, o, True)
+        return [q, k, *back, o]
+
+    want = run()
+    with torch.inference_mode():
+        got = run()
+    assert all(g.is_inference() and torch.equal(g, w) for g, w in zip(got, want))
+
+
 @pytest.mark.parametrize("n", [3, 40])
 def test_calls_at_once_on_two_streams_agree_with_one(n):
     lens = [900, 1300, 5, 0]
