@@ -156,11 +156,6 @@ __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 
 // ---------------------------------------------------------------------------
 // Role: loads and tiles (warps 4-7)
@@ -449,8 +444,8 @@ __device__ __forceinline__ void wide_softmax(const FwdParams4& p, Walk w, char* 
     }
 
     // --- the walk over the tokens ------------------------------------------------------------------------
-    // As in the other kernel: p = 2^(score + off).  The references are whole numbers here, so that rescaling is
-    // exact: a half of P already written may be rescaled in place.
+    // As in the other kernel: p = 2^(score + off).  The references are whole numbers here, so that a half of P already
+    // written may be rescaled in place: exactly, but for products that leave fp16's normal range by it.
     float m_ref = -INFINITY, off = 0.0f, limit_s = -INFINITY, l = 0.0f, e_max = 0.0f, acc_m[kG];
 #pragma unroll
     for (int g = 0; g < kG; ++g) acc_m[g] = 0.0f;
@@ -521,13 +516,15 @@ __device__ __forceinline__ void wide_softmax(const FwdParams4& p, Walk w, char* 
             if (__any_sync(0xffffffffu, by != 1.0f)) {
               if (c == 1 && !twice) {  // this step's first half of P
                 tmem_wait_st();
-                const uint32_t by2 = pack2<false>(by, by);
 #pragma unroll
                 for (int g = 0; g < kG; ++g) {
                   uint32_t x[16];
                   tmem_ld16_sync(mine + g * 64u, x);
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) x[i] = hmul2(x[i], by2);
+                  for (int i = 0; i < 16; ++i) {  // (the factor may be below fp16's range where the product is not)
+                    const float2 f = unpack2<false>(x[i]);
+                    x[i] = pack2<false>(f.x * by, f.y * by);
+                  }
                   tmem_st16(mine + g * 64u, x);
                 }
               }

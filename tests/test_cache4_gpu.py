@@ -367,6 +367,76 @@ def test_negative_steps_are_taken_as_written():
     assert abs(lse.item() - want_lse.item()) <= 2.0 ** -19 * reach + 2.0 ** -15 + 2.0 ** -22 * abs(want_lse.item())
 
 
+# --- values whose steps lie far apart --------------------------------------------------------------------
+def stepped(x, s, d, dtype, seed=0, low=-7.5):
+    """(cache, table) of one sequence and head whose scores are exactly x[t] log2 units (ones_query) and whose values
+    have steps of s[t] to 2 s[t] and minima of `low` steps; a step of 0 stands for the constant 1."""
+    T, G = len(x), d // 64
+    g = torch.Generator().manual_seed(seed)
+    x = x.to(dtype).double()[:, None].expand(T, G)
+    none = torch.zeros(T, G, dtype=torch.float64)
+    s = s.double()[:, None] * (1 + torch.rand(T, G, generator=g).double())
+    s = s.to(dtype).double()
+    m = torch.where(s == 0, torch.ones_like(s), torch.where(torch.isfinite(s), low * s, none))
+    codes = torch.randint(0, 16, (T, d), generator=g) * (s > 0).repeat_interleave(64, -1)
+    table, n_pages = pages([T], 16, seed)
+    cache, t = noise_cache(n_pages, 1, 16, d, seed), torch.arange(T)
+    cache[table[0, t // 16].long(), 0, 0, t % 16] = oc.pack_rows(torch.zeros(T, d, dtype=torch.long), none, x, dtype)
+    cache[table[0, t // 16].long(), 0, 1, t % 16] = oc.pack_rows(codes, s, m, dtype)
+    return cache, table
+
+
+def ones_query(n, d, dtype):
+    # two heads; at scale ln 2 the first one's scores are the keys' constants, the second one's half of them
+    return torch.tensor([1.0, 0.5])[:, None].expand(1, n, 2, d).to(dtype) / d
+
+
+def check_steps(q, cache, table, T, causal, rows=None):
+    """As check_attention, for steps of any size.  Products p s' far below a row's largest keep fewer bits: the largest
+    stands at 2^7 or more of fp16, whose smallest step is 2^-24, so each is off by 2^-32 of it beside 2^-11 relative
+    (in the kernel for many rows twice, where a reference moves within a step), times a code of at most 15: T 2^-27.
+    The two fp32 sums pass 15 times the largest and are rounded, towards zero even, twice in 16 tokens: T 2^-22."""
+    n = q.shape[1]
+    rows = list(range(n)) if rows is None else rows
+    o, lse = fa.forward_cache4(q.cuda(), cache.cuda(), table.cuda(), ints([T]).cuda(), None, causal, math.log(2), True)
+    fa.check_status(0)
+    o, lse = o.cpu().double(), lse.cpu().double()
+    d, dtype = q.shape[3], q.dtype
+    kr, vr = oc.sequence_rows(cache, table, 0, T)[:, :, 0]
+    key = oc.unpack_rows(kr, dtype)[2][:, 0]
+    codes, s, m = oc.unpack_rows(vr, dtype)
+    for i in rows:
+        see = T - n + i + 1 if causal else T
+        for h in range(2):
+            score = key[:see] * (1.0, 0.5)[h]  # log2 units
+            p = torch.softmax(score * math.log(2), 0)
+            part, low = codes[:see] * s[:see].repeat_interleave(64, -1), m[:see].repeat_interleave(64, -1)
+            want, weight = p @ (part + low), p @ (part + low.abs())
+            largest = (p[:, None] * s[:see]).max()
+            reach = float(score.abs().max()) * math.log(2)
+            tol = want.abs() * torch.finfo(dtype).eps / 2 + (2.0 ** -11 + 2.0 ** -18 * reach + 2.0 ** -15) * weight + TINY[dtype]
+            tol = tol + see * 2.0 ** -21 * largest
+            err = (o[0, i, h] - want).abs()
+            assert torch.all(err <= tol), f"row {i} head {h}: largest error over tolerance {(err / tol).max().item():.3g}"
+            want = torch.logsumexp(score * math.log(2), 0).item()
+            assert abs(lse[0, h, i].item() - want) <= 2.0 ** -19 * reach + 2.0 ** -15 + 2.0 ** -22 * abs(want)
+
+
+def uneven(T, seed):
+    return torch.rand(T, generator=torch.Generator().manual_seed(seed)) * 2 - 1
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_maximum_that_jumps_between_the_halves_of_a_step(d):
+    # 128 rows: tokens 32 on are 25 log2 units above those before, whose steps are 2^19 times theirs
+    T = 64
+    x, s = torch.zeros(T), torch.ones(T)
+    x[32:] = 25
+    s[:32] = 2.0 ** 19
+    cache, table = stepped(x, s, d, torch.bfloat16, 1, low=0.0)
+    check_steps(ones_query(64, d, torch.bfloat16), cache, table, T, False)
+
+
 # --- lengths and pages that are wrong --------------------------------------------------------------------
 @pytest.mark.parametrize("entry", ["write", "read", "attend", "attend many"])
 @pytest.mark.parametrize("fault", ["page low", "page high", "length high", "length low", "new high", "new low"])
