@@ -10,8 +10,13 @@ namespace afa100 {
 constexpr int kUnit = 128;        // tokens of a unit of work
 constexpr int kItemUnits = 4;     // units an item is charged beside its tokens'
 constexpr int kWholeTokens = 512; // items that cannot be longer are not split, if there is a CTA for each
-constexpr float kRescale = 8.0f;  // log2 units a score may pass the reference maximum by
-constexpr float kHeadroom = 7.0f; // log2 of p s' at the reference maximum and the largest step
+// What a row's weights are measured by, so that p s' fits fp16: its reference is the largest score + log2(size) of the
+// tokens it sees, and p = 2^(score + kHeadroom - reference).  A token's size is its larger step; 2^-20 of its minima
+// and 2^-60 at least, so that p itself and p m' stay far from fp32's largest where there are no steps.
+constexpr float kRescale = 8.0f;   // log2 units the product may pass the reference by
+constexpr float kHeadroom = 7.0f;  // log2 of the product at the reference
+constexpr float kLeastSize = 8.673617379884035e-19f;
+constexpr float kMinimaSize = 9.5367431640625e-07f;
 
 struct FwdParams4 {
   AfaCache4 c;
@@ -41,6 +46,20 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A token's size from one group's step and minimum (above); what is not finite has none.
+__device__ __forceinline__ float size_of(float size, float step, float minimum) {
+  const float a = fabsf(step), b = fabsf(minimum) * kMinimaSize;
+  return fmax3(size, a < INFINITY ? a : 0.0f, b < INFINITY ? b : 0.0f);
+}
+// The power of two above, to 2^126; its logarithm.
+__device__ __forceinline__ float power_above(float x) { return __uint_as_float((min(__float_as_uint(x) >> 23, 252u) + 1u) << 23); }
+__device__ __forceinline__ float log2_of_power(float x) { return static_cast<float>(static_cast<int>(__float_as_uint(x) >> 23) - 127); }
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // p + n * stride bytes

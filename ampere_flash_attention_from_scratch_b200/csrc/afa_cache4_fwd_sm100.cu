@@ -13,9 +13,10 @@
 //
 //   * q is held in fp16 for either type, each row scaled by a power of two so
 //     that its largest element lies in [2^13, 2^14); the product is exact.
-//   * p s' is rounded to fp16: 2^-12 relative, as for a 16-bit P.  A power of two
-//     in the exponent of p keeps the largest product so far below 2^15, which
-//     leaves 2^-31 of it as the smallest that keeps a bit.
+//   * p s' is rounded to fp16: 2^-11 relative, as for a 16-bit P.  The exponent of
+//     p is measured by the largest product p s' of the tokens the row has seen, which
+//     stays between 2^7 and 2^15: products down to 2^-21 of it keep all their bits,
+//     smaller ones are off by 2^-32 of it.
 //   * p, its sum, the running maximum and both accumulators are fp32.
 //
 // Bound.  HBM would be: 1.125 bytes a channel and token for keys and values.  The
@@ -312,16 +313,16 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 || kD == 64 ? 3 : 2) cache4
     if (p.causal) limit_min = min(it.tokens, max(0, it.tokens - fresh + tile * L::kRows / p.group + 1));
 
     // --- the walk over the tokens ------------------------------------------------------------------------
-    // A weight is held as p = 2^(score + off): off takes off the row's reference maximum (none yet: -inf) and the
-    // power of two above the largest step so far, so that p s' stays within 2^(kRescale + kHeadroom).
-    float m_ref[kNT][2], off[kNT][2], limit_s[kNT][2], l[kNT][2];
-    float e_max = 0.0f;
+    // A weight is held as p = 2^(score + off): off takes off the row's reference (none yet: -inf), so that p s' stays
+    // within 2^(kRescale + kHeadroom).
+    float ref[kNT][2], off[kNT][2], limit_s[kNT][2], l[kNT][2];
+    float step_max = 0.0f;
     float acc[kNT][kG][4][4], acc_m[kNT][kG][2];
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        m_ref[nt][x] = limit_s[nt][x] = -INFINITY;
+        ref[nt][x] = limit_s[nt][x] = -INFINITY;
         off[nt][x] = l[nt][x] = 0.0f;
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
@@ -424,48 +425,67 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 || kD == 64 ? 3 : 2) cache4
         }
       }
 
-      // New references only where a score passes the old one by 2^kRescale, or a step the old power of two.
-      bool moved = vs_max > e_max;
-      float top[kNT][2];
+      // A row's reference moves where p s' of a token it sees would pass 2^(kRescale + kHeadroom).  As long as no step
+      // passes step_max (a power of two), no score above limit_s tells that; otherwise the products are looked at.
+      // What a row does not see moves nothing but step_max.
+      bool look = vs_max > step_max;
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          top[nt][x] = fmaxf(s[nt][x], s[nt][2 + x]);
-          moved |= top[nt][x] > limit_s[nt][x];
+        for (int x = 0; x < 2; ++x) look |= fmaxf(s[nt][x], s[nt][2 + x]) > limit_s[nt][x];
+      if (__any_sync(0xffffffffu, look)) {
+        float size[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          size[y] = kLeastSize;
+#pragma unroll
+          for (int gr = 0; gr < kG; ++gr) size[y] = size_of(size[y], vs[y][gr], vm[y][gr]);
         }
-      if (__any_sync(0xffffffffu, moved)) {
-        const float seen = max_over_rows(vs_max);
-        if (seen > e_max) {
-          // the power of two above, from 2^-60 (so that p times a minimum stays far from fp32's largest) to 2^126
-          const uint32_t ex = min(max(__float_as_uint(seen) >> 23, 66u), 252u) + 1u;
-          e_max = __uint_as_float(ex << 23);
-        }
-        const float e = e_max > 0.0f ? static_cast<float>(static_cast<int>(__float_as_uint(e_max) >> 23) - 127) : 0.0f;
+        const float seen = max_over_rows(fmaxf(size[0], size[1]));
+        if (seen > step_max) step_max = power_above(seen);
+        const float limit = kRescale + kHeadroom - log2_of_power(step_max);
+        size[0] = lg2_approx(size[0]);
+        size[1] = lg2_approx(size[1]);
+        float top[kNT][2];
+        bool passes = false;
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const float now = fmaxf(m_ref[nt][x], max_over_rows(top[nt][x] - off[nt][x]));
-            const float to = now == -INFINITY ? 0.0f : kHeadroom - e - now;
-            const float shift = to - off[nt][x];
-            const float by = m_ref[nt][x] == -INFINITY ? 1.0f : ex2_approx(shift);
-            limit_s[nt][x] = now == -INFINITY ? -INFINITY : kRescale + kHeadroom - e;
-            m_ref[nt][x] = now;
-            off[nt][x] = to;
-            s[nt][x] += shift;
-            s[nt][2 + x] += shift;
-            l[nt][x] *= by;
+            top[nt][x] = fmaxf(s[nt][x] + size[0], s[nt][2 + x] + size[1]);
+            passes |= top[nt][x] > (ref[nt][x] == -INFINITY ? -INFINITY : kRescale + kHeadroom);
+            if (ref[nt][x] != -INFINITY) limit_s[nt][x] = limit;
+          }
+        if (__any_sync(0xffffffffu, passes)) {
 #pragma unroll
-            for (int gr = 0; gr < kG; ++gr) {
-              acc_m[nt][gr][x] *= by;
+          for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-              for (int mt = 0; mt < 4; ++mt) {
-                acc[nt][gr][mt][x] *= by;
-                acc[nt][gr][mt][2 + x] *= by;
+            for (int x = 0; x < 2; ++x) {
+              const float most = max_over_rows(top[nt][x]);
+              const bool none = ref[nt][x] == -INFINITY;
+              const bool pass = most > (none ? -INFINITY : kRescale + kHeadroom);
+              const float to = pass ? kHeadroom - (most - off[nt][x]) : off[nt][x], shift = to - off[nt][x];
+              // as a square, since steps that grow by more than 2^126 leave weights that still count
+              const float by = none ? 1.0f : ex2_approx(0.5f * shift);
+              if (pass) {
+                limit_s[nt][x] = limit;
+                ref[nt][x] = most - off[nt][x];
+              }
+              off[nt][x] = to;
+              s[nt][x] += shift;
+              s[nt][2 + x] += shift;
+              l[nt][x] = l[nt][x] * by * by;
+#pragma unroll
+              for (int gr = 0; gr < kG; ++gr) {
+                acc_m[nt][gr][x] = acc_m[nt][gr][x] * by * by;
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt) {
+                  acc[nt][gr][mt][x] = acc[nt][gr][mt][x] * by * by;
+                  acc[nt][gr][mt][2 + x] = acc[nt][gr][mt][2 + x] * by * by;
+                }
               }
             }
-          }
+        }
       }
 
       const char* vb = kb + L::kSideBytes;
@@ -562,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 || kD == 64 ? 3 : 2) cache4
         const int row = nt * 8 + 2 * t + x;
         const float sum = sum_over_rows(l[nt][x]);
         if (g == 0) {
-          stats[(warp * L::kRows + row) * 2] = m_ref[nt][x] == -INFINITY ? -INFINITY : -off[nt][x];
+          stats[(warp * L::kRows + row) * 2] = ref[nt][x] == -INFINITY ? -INFINITY : -off[nt][x];
           stats[(warp * L::kRows + row) * 2 + 1] = sum;
         }
 #pragma unroll
@@ -593,13 +613,14 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 || kD == 64 ? 3 : 2) cache4
       float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll
       for (int v = 0; v < kWarps; ++v) {
-        const float by = m[v] == -INFINITY && top == -INFINITY ? 1.0f : ex2_approx(m[v] - top);
-        sum = fmaf(by, stats[(v * L::kRows + row) * 2 + 1], sum);
+        // a square, as above
+        const float by = m[v] == -INFINITY && top == -INFINITY ? 1.0f : ex2_approx(0.5f * (m[v] - top));
+        sum = fmaf(by, by * stats[(v * L::kRows + row) * 2 + 1], sum);
         const float4 f = *reinterpret_cast<const float4*>(smem + places[v] + (row * kD + c4 * 4) * 4);
-        o.x = fmaf(by, f.x, o.x);
-        o.y = fmaf(by, f.y, o.y);
-        o.z = fmaf(by, f.z, o.z);
-        o.w = fmaf(by, f.w, o.w);
+        o.x = fmaf(by, by * f.x, o.x);
+        o.y = fmaf(by, by * f.y, o.y);
+        o.z = fmaf(by, by * f.z, o.z);
+        o.w = fmaf(by, by * f.w, o.w);
       }
       const int r = tile * L::kRows + row;
       if (whole) {
@@ -670,14 +691,16 @@ __global__ void __launch_bounds__(128) cache4_join_kernel(const FwdParams4 p) {
     const float* sh = share(i);
     const float2 ml = *reinterpret_cast<const float2*>(sh + L::kRows * kD + row * 2);
     const float now = fmaxf(top, ml.x);
-    const float old = now == -INFINITY ? 1.0f : ex2_approx(top - now), by = now == -INFINITY ? 1.0f : ex2_approx(ml.x - now);
+    // (squares of these, as in the first kernel)
+    const float old = now == -INFINITY ? 1.0f : ex2_approx(0.5f * (top - now));
+    const float by = now == -INFINITY ? 1.0f : ex2_approx(0.5f * (ml.x - now));
     top = now;
-    sum = fmaf(by, ml.y, sum * old);
+    sum = fmaf(by, by * ml.y, sum * old * old);
 #pragma unroll
     for (int x = 0; x < kPer; x += 2) {
       const float2 v = *reinterpret_cast<const float2*>(sh + row * kD + lane * kPer + x);
-      o[x] = fmaf(by, v.x, o[x] * old);
-      o[x + 1] = fmaf(by, v.y, o[x + 1] * old);
+      o[x] = fmaf(by, by * v.x, o[x] * old * old);
+      o[x + 1] = fmaf(by, by * v.y, o[x + 1] * old * old);
     }
   }
   const int n = r / p.group, h = head * p.group + (r - n * p.group);

@@ -446,7 +446,7 @@ __device__ __forceinline__ void wide_softmax(const FwdParams4& p, Walk w, char* 
     // --- the walk over the tokens ------------------------------------------------------------------------
     // As in the other kernel: p = 2^(score + off).  The references are whole numbers here, so that a half of P already
     // written may be rescaled in place: exactly, but for products that leave fp16's normal range by it.
-    float m_ref = -INFINITY, off = 0.0f, limit_s = -INFINITY, l = 0.0f, e_max = 0.0f, acc_m[kG];
+    float reference = -INFINITY, off = 0.0f, limit_s = -INFINITY, l = 0.0f, step_max = 0.0f, acc_m[kG];
 #pragma unroll
     for (int g = 0; g < kG; ++g) acc_m[g] = 0.0f;
     const int limit = p.causal ? min(it.tokens, max(0, it.tokens - fresh + n + 1)) : it.tokens;
@@ -461,12 +461,7 @@ __device__ __forceinline__ void wide_softmax(const FwdParams4& p, Walk w, char* 
         const float* vs = reinterpret_cast<const float*>(smem + L::kOffVs);
         const float4 big = *reinterpret_cast<const float4*>(smem + L::kOffSeen);
         const float seen = kG == 2 ? fmaxf(fmaxf(big.x, big.y), fmaxf(big.z, big.w)) : fmaxf(big.x, big.y);
-        bool grow = seen > e_max;
-        if (grow) {
-          const uint32_t ex = min(max(__float_as_uint(seen) >> 23, 66u), 252u) + 1u;
-          e_max = __uint_as_float(ex << 23);
-        }
-        const float e = e_max > 0.0f ? static_cast<float>(static_cast<int>(__float_as_uint(e_max) >> 23) - 127) : 0.0f;
+        bool grow = seen > step_max;
         // 32 tokens
         auto half = [&](auto masked_tag, const int c) {
           constexpr bool kMasked = decltype(masked_tag)::value;
@@ -500,45 +495,66 @@ __device__ __forceinline__ void wide_softmax(const FwdParams4& p, Walk w, char* 
 #pragma unroll
           for (int i = 0; i < 32; i += 2) top = fmax3(top, v[i], v[i + 1]);
 
+          // (as in the other kernel; a lane finds the size of one token, for all rows)
           if (__any_sync(0xffffffffu, grow || top > limit_s)) {
-            const float now = fmaxf(m_ref, ceilf(top - off));
-            const float to = now == -INFINITY ? 0.0f : kHeadroom - e - now;
-            const float move = to - off;
-            const float by = m_ref == -INFINITY ? 1.0f : ex2_approx(move);
-            limit_s = now == -INFINITY ? -INFINITY : kRescale + kHeadroom - e;
-            m_ref = now;
-            off = to;
+            const float* mine_vs = vs + (32 * c + lane) * 2 * kG;
+            float size = kLeastSize;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += move;
-            l *= by;
+            for (int g = 0; g < kG; ++g) size = size_of(size, mine_vs[g], mine_vs[kG + g]);
+            float most = fmaxf(size, seen);
 #pragma unroll
-            for (int g = 0; g < kG; ++g) acc_m[g] *= by;
-            if (__any_sync(0xffffffffu, by != 1.0f)) {
-              if (c == 1 && !twice) {  // this step's first half of P
-                tmem_wait_st();
+            for (int x = 1; x < 32; x <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+            if (most > step_max) step_max = power_above(most);
+            const float limit = kRescale + kHeadroom - log2_of_power(step_max);
+            size = lg2_approx(size);
+            most = -INFINITY;
 #pragma unroll
-                for (int g = 0; g < kG; ++g) {
-                  uint32_t x[16];
-                  tmem_ld16_sync(mine + g * 64u, x);
+            for (int i = 0; i < 32; ++i) most = fmaxf(most, v[i] + __shfl_sync(0xffffffffu, size, i));
+            const bool none = reference == -INFINITY;
+            const bool passes = most > (none ? -INFINITY : kRescale + kHeadroom);
+            if (!none || passes) limit_s = limit;
+            if (__any_sync(0xffffffffu, passes)) {
+              const float now = passes ? ceilf(most - off) : reference;
+              const float to = passes ? kHeadroom - now : off;
+              const float move = to - off;
+              // in two parts, since steps that grow by more than 2^126 leave weights that still count
+              const float part = truncf(0.5f * move);
+              const float by0 = none ? 1.0f : ex2_approx(part), by1 = none ? 1.0f : ex2_approx(move - part);
+              reference = now;
+              off = to;
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) {  // (the factor may be below fp16's range where the product is not)
-                    const float2 f = unpack2<false>(x[i]);
-                    x[i] = pack2<false>(f.x * by, f.y * by);
+              for (int i = 0; i < 32; ++i) v[i] += move;
+              l = l * by0 * by1;
+#pragma unroll
+              for (int g = 0; g < kG; ++g) acc_m[g] = acc_m[g] * by0 * by1;
+              if (__any_sync(0xffffffffu, by1 != 1.0f)) {
+                // (rolled loops: a step's code has to stay in the instruction cache, 2851 us for the chunk above, else 2938)
+                if (c == 1 && !twice) {  // this step's first half of P
+                  tmem_wait_st();
+#pragma unroll 1
+                  for (int g = 0; g < kG; ++g) {
+                    uint32_t x[16];
+                    tmem_ld16_sync(mine + g * 64u, x);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {  // (a factor may be below fp16's range where the product is not)
+                      const float2 f = unpack2<false>(x[i]);
+                      x[i] = pack2<false>(f.x * by0 * by1, f.y * by0 * by1);
+                    }
+                    tmem_st16(mine + g * 64u, x);
                   }
-                  tmem_st16(mine + g * 64u, x);
                 }
-              }
-              if (!first) {
+                if (!first) {
+#pragma unroll 1
+                  for (int o = 0; o < kD; o += 16) {
+                    uint32_t x[16];
+                    tmem_ld16_sync(mine + L::kColO + o, x);
 #pragma unroll
-                for (int o = 0; o < kD; o += 16) {
-                  uint32_t x[16];
-                  tmem_ld16_sync(mine + L::kColO + o, x);
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * by);
-                  tmem_st16(mine + L::kColO + o, x);
+                    for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * by0 * by1);
+                    tmem_st16(mine + L::kColO + o, x);
+                  }
                 }
+                tmem_wait_st();
               }
-              tmem_wait_st();
             }
             grow = false;
           }
@@ -609,7 +625,7 @@ __device__ __forceinline__ void wide_softmax(const FwdParams4& p, Walk w, char* 
     // A wait that ran out for one warp is everyone's here: the four leave at the same barrier.
     ok = agree<2>(ok);
     if (!ok) break;
-    float ref = m_ref == -INFINITY ? -INFINITY : -off;
+    float ref = reference == -INFINITY ? -INFINITY : -off;
     // Q's tile is free now and holds the second copies' rows of O: 16-byte piece c of row r at c ^ (r mod 8).
     auto second = [&](int c) {
       return reinterpret_cast<float4*>(smem + L::kOffQ + row * (kD * 4) + ((c & ~7) | ((c ^ row) & 7)) * 16);
@@ -641,9 +657,9 @@ __device__ __forceinline__ void wide_softmax(const FwdParams4& p, Walk w, char* 
       if (copy == 0 && valid) {
         const float2 s = ml[row];
         const float both = fmaxf(ref, s.x);
-        by = both == -INFINITY ? 1.0f : ex2_approx(ref - both);
-        by_second = both == -INFINITY ? 1.0f : ex2_approx(s.x - both);
-        l = fmaf(by_second, s.y, l * by);
+        by = both == -INFINITY ? 1.0f : ex2_approx(0.5f * (ref - both));  // squares of these, as above
+        by_second = both == -INFINITY ? 1.0f : ex2_approx(0.5f * (s.x - both));
+        l = fmaf(by_second, by_second * s.y, l * by * by);
         ref = both;
       }
     }
@@ -669,7 +685,7 @@ __device__ __forceinline__ void wide_softmax(const FwdParams4& p, Walk w, char* 
             const float4 s0 = *second(2 * c), s1 = *second(2 * c + 1);
             const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = fmaf(by_second, s[i], f[i] * by);
+            for (int i = 0; i < 8; ++i) f[i] = fmaf(by_second, by_second * s[i], f[i] * by * by);
           }
           if (whole) {
             uint4 out = make_uint4(0, 0, 0, 0);

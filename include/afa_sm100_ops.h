@@ -127,9 +127,12 @@ int afa_cache4_read_sm100(const AfaCache4* cache, void* k, void* v, const int64_
  * afa_fwd_sm100.  causal: row i sees the tokens up to its own position
  * kv_lens[b] - new_lens[b] + i.  A row that sees no token and a padding row
  * get O = 0 and lse = -inf.  A NaN among a row's visible keys makes the row NaN,
- * one among its visible values the 64 channels of its group; one that is masked
- * does nothing.  Queries are exact up to 2^110 in magnitude, values' steps up to
- * 2^100.  Calls of more than 64 query rows a key/value head (seq_len * n_heads /
+ * one among its visible values the 64 channels of its group; a masked token does
+ * nothing, whatever it holds.  Queries are exact up to 2^110 in magnitude.  A
+ * token's weight times each of its two values' steps is held in fp16, measured by
+ * the largest such product of the row: 2^-11 relative down to 2^-21 of that, and
+ * below to 2^-32 of it.  Steps may go up to 2^100; where all of a row's lie below
+ * 2^-81 they lose bits.  Calls of more than 64 query rows a key/value head (seq_len * n_heads /
  * n_kv_heads) run on tcgen05, others on mma.sync. */
 typedef struct AfaCache4FwdArgs {
   const void* q;

@@ -392,10 +392,12 @@ def ones_query(n, d, dtype):
 
 
 def check_steps(q, cache, table, T, causal, rows=None):
-    """As check_attention, for steps of any size.  Products p s' far below a row's largest keep fewer bits: the largest
-    stands at 2^7 or more of fp16, whose smallest step is 2^-24, so each is off by 2^-32 of it beside 2^-11 relative
-    (in the kernel for many rows twice, where a reference moves within a step), times a code of at most 15: T 2^-27.
-    The two fp32 sums pass 15 times the largest and are rounded, towards zero even, twice in 16 tokens: T 2^-22."""
+    """As check_attention, for steps of any size.  The rounded p s' multiplies a code with a mean taken off, which is 15
+    at most in magnitude and which the other sum gives back: both sums' terms reach p (15 s' + |m'|).  Products far
+    below a row's largest keep fewer bits: the largest stands at 2^7 or more of fp16, whose smallest step is 2^-24, so
+    each is off by 2^-32 of it beside 2^-11 relative (in the kernel for many rows twice, where a reference moves within
+    a step), times 15: T 2^-27.  The fp32 sums pass 15 times the largest and are rounded, towards zero even, twice in
+    16 tokens: T 2^-22."""
     n = q.shape[1]
     rows = list(range(n)) if rows is None else rows
     o, lse = fa.forward_cache4(q.cuda(), cache.cuda(), table.cuda(), ints([T]).cuda(), None, causal, math.log(2), True)
@@ -410,8 +412,8 @@ def check_steps(q, cache, table, T, causal, rows=None):
         for h in range(2):
             score = key[:see] * (1.0, 0.5)[h]  # log2 units
             p = torch.softmax(score * math.log(2), 0)
-            part, low = codes[:see] * s[:see].repeat_interleave(64, -1), m[:see].repeat_interleave(64, -1)
-            want, weight = p @ (part + low), p @ (part + low.abs())
+            step, low = s[:see].repeat_interleave(64, -1), m[:see].repeat_interleave(64, -1)
+            want, weight = p @ (codes[:see] * step + low), p @ (15 * step + low.abs())
             largest = (p[:, None] * s[:see]).max()
             reach = float(score.abs().max()) * math.log(2)
             tol = want.abs() * torch.finfo(dtype).eps / 2 + (2.0 ** -11 + 2.0 ** -18 * reach + 2.0 ** -15) * weight + TINY[dtype]
@@ -435,6 +437,52 @@ def test_a_maximum_that_jumps_between_the_halves_of_a_step(d):
     s[:32] = 2.0 ** 19
     cache, table = stepped(x, s, d, torch.bfloat16, 1, low=0.0)
     check_steps(ones_query(64, d, torch.bfloat16), cache, table, T, False)
+
+
+@pytest.mark.parametrize("dtype,ratio", [(torch.bfloat16, 2.0 ** 24), (torch.bfloat16, 2.0 ** 30), (torch.bfloat16, 2.0 ** 90),
+                                         (torch.float16, 2.0 ** 28), (torch.bfloat16, math.inf)])
+@pytest.mark.parametrize("n,d", [(4, 128), (8, 64), (45, 128), (45, 64), (33, 128)])
+def test_large_steps_in_masked_places_stay_there(n, d, dtype, ratio):
+    # the last three tokens' steps are out of all proportion; rows that do not see them keep every bit
+    T = 50
+    s = torch.full((T,), 2.0 ** -14 if dtype == torch.float16 else 1.0)
+    s[-3:] *= ratio
+    cache, table = stepped(uneven(T, n), s, d, dtype, 2)
+    check_steps(ones_query(n, d, dtype), cache, table, T, True, rows=range(n - 3))
+
+
+@pytest.mark.parametrize("gap,ratio", [(58, 2.0 ** 24), (58, 2.0 ** 40), (40, 2.0 ** 60), (100, 2.0 ** 95), (12, 2.0 ** 20)])
+@pytest.mark.parametrize("n,d", [(1, 128), (3, 64), (45, 128), (45, 64), (33, 128)])
+@pytest.mark.parametrize("T,at", [(100, 0), (100, 37), (3000, 5)])
+def test_a_large_step_of_little_weight(T, at, n, d, gap, ratio):
+    # one token's step is far above the others' and its score far below: what they lose is measured by its product
+    x, s = uneven(T, n), torch.ones(T)
+    x[at] = -gap
+    s[at] = ratio
+    cache, table = stepped(x, s, d, torch.bfloat16, 3)
+    check_steps(ones_query(n, d, torch.bfloat16), cache, table, T, False)
+
+
+@pytest.mark.parametrize("n,d", [(1, 128), (3, 64), (45, 128), (45, 64), (33, 128)])
+@pytest.mark.parametrize("T,at", [(131, 130), (40, 39), (2000, 1999)])
+def test_constant_values_before_a_large_step(T, at, n, d):
+    # values without a step, then one of 2^100 and a weight of 2^-10: the first ones' weights stay in the sum
+    x, s = torch.zeros(T), torch.zeros(T)
+    x[at] = -10
+    s[at] = 2.0 ** 100
+    cache, table = stepped(x, s, d, torch.bfloat16, 4, low=0.0)
+    check_steps(ones_query(n, d, torch.bfloat16), cache, table, T, False)
+
+
+@pytest.mark.parametrize("n,d", [(2, 128), (40, 64)])
+def test_steps_that_rise_and_fall(n, d):
+    # products move over 2^80 along the sequence in both directions, the scores against them
+    T = 1500
+    t = torch.arange(T).double()
+    s = 2.0 ** (40 * torch.sin(t / 90)).float()
+    x = (30 * torch.cos(t / 50)).float()
+    cache, table = stepped(x, s, d, torch.bfloat16, 5)
+    check_steps(ones_query(n, d, torch.bfloat16), cache, table, T, True)
 
 
 # --- lengths and pages that are wrong --------------------------------------------------------------------
