@@ -172,6 +172,11 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
     variable_list out = rotary_new(q, k.has_value() ? *k : at::Tensor(), positions, inv_freq,
                                    RotaryPlan{sections, interleaved, inverse});
     if (!k.has_value()) out.pop_back();
+    // an output follows its own input only
+    variable_list constant;
+    if (!q.requires_grad()) constant.push_back(out[0]);
+    if (k.has_value() && !k->requires_grad()) constant.push_back(out[1]);
+    if (!constant.empty()) ctx->mark_non_differentiable(constant);
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {

@@ -162,6 +162,21 @@ def test_gradient_of_shared_and_broadcast_inputs():
     assert torch.equal(gy, one.sum(0, keepdim=True))
 
 
+@pytest.mark.parametrize("trained", ["q", "k"])
+def test_an_output_requires_a_gradient_if_its_input_does(trained):
+    g = torch.Generator().manual_seed(7)
+    q, k, up = (torch.randn(2, 6, 3, 64, generator=g).half().cuda() for _ in range(3))
+    pos, inv = torch.arange(12).view(1, 2, 6).cuda(), _inv(32).cuda()
+    x = (q if trained == "q" else k).requires_grad_()
+    out = fa.rotary(q, k, pos, inv)
+    ours, other = out if trained == "q" else out[::-1]
+    assert ours.requires_grad and not other.requires_grad and other.grad_fn is None
+    (gx,) = torch.autograd.grad(ours, x, up)
+    assert torch.equal(gx, fa.rotary(up, None, pos, inv, inverse=True)[0])
+    plain = fa.rotary(q.detach(), k.detach(), pos, inv)
+    assert torch.equal(out[0], plain[0]) and torch.equal(out[1], plain[1])
+
+
 def test_capture_of_forward_and_backward():
     g = torch.Generator().manual_seed(6)
     q, dq = (torch.randn(2, 100, 4, 128, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
