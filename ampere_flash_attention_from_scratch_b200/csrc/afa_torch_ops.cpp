@@ -197,8 +197,36 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
   }
 };
 
+// Whether forward-mode differentiation follows t.
+bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+
+// Forward mode: a rotation is linear, so an output's tangent is its input's tangent turned alike.
+variable_list rotary_dual(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                          const at::Tensor& inv_freq, const RotaryPlan& plan) {
+  at::Tensor x[2], dx[2];
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor& t = i == 0 ? q : k;
+    if (!t.defined()) continue;
+    std::tie(x[i], dx[i]) = at::_unpack_dual(t, 0);
+    if (dx[i].defined()) dx[i] = dx[i]._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : as_rows(dx[i]);
+  }
+  variable_list out = rotary_any(x[0], x[1], positions, inv_freq, plan);
+  at::Tensor d[2];
+  if (dx[0].defined()) {
+    const variable_list turned = rotary_any(dx[0], dx[1], positions, inv_freq, plan);
+    d[0] = turned[0];
+    d[1] = turned[1];
+  } else {
+    d[1] = rotary_any(dx[1], at::Tensor(), positions, inv_freq, plan)[0];
+  }
+  for (int i = 0; i < 2; ++i)
+    if (d[i].defined()) out[i] = at::_make_dual(out[i], d[i], 0);
+  return out;
+}
+
 variable_list rotary_any(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
                          const at::Tensor& inv_freq, const RotaryPlan& plan) {
+  if (has_tangent(q) || has_tangent(k)) return rotary_dual(q, k, positions, inv_freq, plan);
   if (at::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
     const std::optional<at::Tensor> second = k.defined() ? std::optional<at::Tensor>(k) : std::nullopt;
     variable_list out =
@@ -249,7 +277,8 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> rotary(const at::Tensor& q, co
   }
   TORCH_CHECK(sum == pairs, "sections must add up to the ", pairs, " pairs of inv_freq (got ", sum, ")");
   const bool grad = at::GradMode::is_enabled();
-  TORCH_CHECK(!grad || (!positions.requires_grad() && !inv_freq.requires_grad()),
+  TORCH_CHECK((!grad || (!positions.requires_grad() && !inv_freq.requires_grad())) && !has_tangent(positions) &&
+                  !has_tangent(inv_freq),
               "positions and inv_freq are not differentiable");
   const bool out_given = (q_out_.has_value() && q_out_->defined()) || (k_out_.has_value() && k_out_->defined());
   TORCH_CHECK(k.defined() || !k_out_.has_value() || !k_out_->defined(), "k_out without k");
@@ -259,12 +288,13 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> rotary(const at::Tensor& q, co
   raise_earlier_abort(q.device().index());
   variable_list out;
   if (out_given) {
-    TORCH_CHECK(!grad || !(q.requires_grad() || (k.defined() && k.requires_grad())),
-                "q_out and k_out cannot be given for inputs that require a gradient");
+    TORCH_CHECK((!grad || !(q.requires_grad() || (k.defined() && k.requires_grad()))) && !has_tangent(q) && !has_tangent(k),
+                "q_out and k_out cannot be given for inputs that require a gradient or have a tangent");
     const at::Tensor q_out = output_like(q_out_, q, "q_out");
     const at::Tensor k_out = k.defined() ? output_like(k_out_, k, "k_out") : at::Tensor();
-    TORCH_CHECK(!grad || !(q_out.requires_grad() || (k_out.defined() && k_out.requires_grad())),
-                "q_out and k_out must not require a gradient");
+    TORCH_CHECK((!grad || !(q_out.requires_grad() || (k_out.defined() && k_out.requires_grad()))) &&
+                    !has_tangent(q_out) && !has_tangent(k_out),
+                "q_out and k_out must not require a gradient or have a tangent");
     rotary_launch(q, k, q_out, k_out, positions, inv_freq, plan);
     written(q_out);
     if (k_out.defined()) written(k_out);

@@ -177,6 +177,48 @@ def test_an_output_requires_a_gradient_if_its_input_does(trained):
     assert torch.equal(out[0], plain[0]) and torch.equal(out[1], plain[1])
 
 
+def test_tangents():
+    # forward mode: each output's tangent is its input's, turned; with one, the other or both, and through a graph
+    import torch.autograd.forward_ad as fwd
+
+    g = torch.Generator().manual_seed(8)
+    q, k, dq, dk, up = (torch.randn(2, 6, 3, 64, generator=g).half().cuda() for _ in range(5))
+    pos, inv = torch.arange(24).view(2, 2, 6).cuda(), _inv(24).cuda()
+    turn = lambda x: fa.rotary(x, None, pos, inv, [10, 14], True)[0]
+    tangent = lambda x: fwd.unpack_dual(x).tangent
+    with fwd.dual_level():
+        a, b = fa.rotary(fwd.make_dual(q, dq), fwd.make_dual(k, dk), pos, inv, [10, 14], True)
+        assert torch.equal(tangent(a), turn(dq)) and torch.equal(tangent(b), turn(dk))
+        assert torch.equal(fwd.unpack_dual(a).primal, turn(q)) and torch.equal(fwd.unpack_dual(b).primal, turn(k))
+        a, b = fa.rotary(fwd.make_dual(q, dq), k, pos, inv, [10, 14], True)
+        assert torch.equal(tangent(a), turn(dq)) and tangent(b) is None
+        a, b = fa.rotary(q, fwd.make_dual(k, dk), pos, inv, [10, 14], True)
+        assert tangent(a) is None and torch.equal(tangent(b), turn(dk))
+        with torch.no_grad():  # which is about the other mode
+            assert torch.equal(tangent(turn(fwd.make_dual(q, dq))), turn(dq))
+        # a tangent that repeats, and one of zeros without memory
+        assert torch.equal(tangent(turn(fwd.make_dual(q, dq[:1, :1].expand_as(q)))), turn(dq[:1, :1].expand_as(q).contiguous()))
+        assert not tangent(turn(fwd.make_dual(q, torch._efficientzerotensor(q.shape, dtype=q.dtype, device="cuda")))).any()
+        # in both modes at once: gradients of the output and of its tangent
+        x, t = q.clone().requires_grad_(), dq.clone().requires_grad_()
+        a = turn(fwd.make_dual(x, t))
+        assert torch.equal(torch.autograd.grad(a, x, up, retain_graph=True)[0], fa.rotary(up, None, pos, inv, [10, 14], True, True)[0])
+        assert torch.equal(torch.autograd.grad(tangent(a), t, up)[0], fa.rotary(up, None, pos, inv, [10, 14], True, True)[0])
+        # and through the gradient: the tangent of a gradient is the upstream gradient's, turned back
+        gx = torch.autograd.grad(turn(x), x, fwd.make_dual(up, dk), create_graph=True)[0]
+        assert torch.equal(tangent(gx), fa.rotary(dk, None, pos, inv, [10, 14], True, True)[0])
+        for kwargs in (dict(q_out=torch.empty_like(q)), dict(inv_freq=fwd.make_dual(inv, inv))):
+            with pytest.raises(RuntimeError, match="tangent|not differentiable"):
+                fa.rotary(**{**dict(q=fwd.make_dual(q, dq), k=None, positions=pos, inv_freq=inv, sections=[10, 14]), **kwargs})
+        with pytest.raises(RuntimeError, match="must not"):
+            fa.rotary(q, None, pos, inv, [10, 14], q_out=fwd.make_dual(q.clone(), dq))
+    # linear: differences along the tangent in 64 bits
+    want = oc.rotary64(dq.cpu(), pos.cpu(), inv.cpu(), [10, 14], True)
+    diff = oc.rotary64((q.double() + dq.double()).cpu(), pos.cpu(), inv.cpu(), [10, 14], True) - oc.rotary64(q.cpu(), pos.cpu(), inv.cpu(), [10, 14], True)
+    assert torch.allclose(want, diff, atol=1e-12)
+    _check(turn(dq).cpu(), dq.cpu(), want, 48, True)
+
+
 def test_capture_of_forward_and_backward():
     g = torch.Generator().manual_seed(6)
     q, dq = (torch.randn(2, 100, 4, 128, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
