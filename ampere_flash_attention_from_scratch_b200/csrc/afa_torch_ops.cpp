@@ -70,6 +70,15 @@ void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// Whether forward-mode differentiation follows t.
+bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+
+// Tensors of an operator without a gradient: what autograd would follow is refused, since its graph would end there.
+void check_constant(const at::Tensor& t, const char* name, const char* op) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()) && !has_tangent(t), op, " is not differentiable: ", name,
+              " must not require a gradient or have a tangent (detach it, or call under torch.no_grad())");
+}
+
 // `out` if given (checked against `like`), else a new contiguous tensor.
 at::Tensor output_like(const std::optional<at::Tensor>& out, const at::Tensor& like, const char* name) {
   if (!out.has_value() || !out->defined()) return fresh_tensor(like.sizes(), like.scalar_type(), like.device());
@@ -196,9 +205,6 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
     return {dq, dk, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
-
-// Whether forward-mode differentiation follows t.
-bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 
 // Forward mode: a rotation is linear, so an output's tangent is its input's tangent turned alike.
 variable_list rotary_dual(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
@@ -395,6 +401,8 @@ void cache4_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ca
   TORCH_CHECK(v.device() == k.device() && cache.device() == k.device(), "Input tensors must be on the same device");
   TORCH_CHECK(k.sizes() == v.sizes(), "key and value tensors must have the same shape");
   check_positive(k, "k");
+  check_constant(k, "k", "cache4_write");
+  check_constant(v, "v", "cache4_write");
   const AfaCache4 c = cache_args(cache, page_table, kv_lens, new_lens, k.size(0), dtype_code(k));
   TORCH_CHECK(k.size(2) == c.n_kv_heads && k.size(3) == c.head_dim, "k and v [batch, seq, ", k.size(2), ", ", k.size(3),
               "] do not match the cache's ", c.n_kv_heads, " heads of head_dim ", c.head_dim);
@@ -431,6 +439,7 @@ std::tuple<at::Tensor, at::Tensor> cache4_read(const at::Tensor& cache, const at
     TORCH_CHECK(o.device() == cache.device() && o.scalar_type() == dtype && o.dim() == 4 && o.sizes() == at::IntArrayRef(shape) &&
                     o.stride(3) == 1,
                 name, " must be [batch, n, kv_heads, head_dim] of the given dtype on the cache's device, with a contiguous head_dim");
+    check_constant(o, name, "cache4_read");
     return o;
   };
   const at::Tensor k = make(k_out, "k_out"), v = make(v_out, "v_out");
@@ -459,6 +468,7 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> forward_cache4(
   TORCH_CHECK(dtype_code(q) > 0, "Only fp16 and bf16 are supported");
   TORCH_CHECK(cache.device() == q.device(), "Input tensors must be on the same device");
   check_positive(q, "q");
+  check_constant(q, "q", "forward_cache4");
   const AfaCache4 c = cache_args(cache, page_table, kv_lens, new_lens, q.size(0), dtype_code(q));
   TORCH_CHECK(q.size(3) == c.head_dim, "query head_dim (", q.size(3), ") and the cache's (", c.head_dim, ") differ");
   TORCH_CHECK(q.size(2) % c.n_kv_heads == 0, "the number of query heads (", q.size(2),
@@ -470,6 +480,7 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> forward_cache4(
     TORCH_CHECK(static_cast<float>(scale) > 0.0f && scale < 1e38, "softmax_scale ", scale, " is not one of fp32's range");
   }
   const at::Tensor o = output_like(o_, q, "o");
+  check_constant(o, "o", "forward_cache4");
   const int32_t n = static_cast<int32_t>(q.size(1)), heads = static_cast<int32_t>(q.size(2));
   std::optional<at::Tensor> lse;
   if (return_lse)

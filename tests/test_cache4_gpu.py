@@ -581,6 +581,31 @@ def test_refusals():
     fa.check_status(0)
 
 
+def test_what_autograd_follows_is_refused():
+    # the three operators have no gradient: inputs and given outputs that ask for one are refused, not cut off
+    import torch.autograd.forward_ad as fwd
+
+    cache = torch.zeros(4, 2, 2, 16, 36, dtype=torch.uint8, device="cuda")
+    x = torch.ones(2, 3, 2, 64, dtype=torch.float16, device="cuda")
+    table, lens = ints([[0, 1], [2, 3]]).cuda(), ints([20, 30]).cuda()
+    calls = [lambda t: fa.forward_cache4(t, cache, table, lens), lambda t: fa.forward_cache4(x, cache, table, lens, t),
+             lambda t: fa.cache4_write(t, x, cache, table, lens), lambda t: fa.cache4_write(x, t, cache, table, lens),
+             lambda t: fa.cache4_read(cache, table, lens, 3, torch.float16, None, t),
+             lambda t: fa.cache4_read(cache, table, lens, 3, torch.float16, None, None, t)]
+    trained = x.clone().requires_grad_()
+    for call in calls:
+        for t in (trained, trained * 2):
+            with pytest.raises(RuntimeError, match="not differentiable"):
+                call(t)
+            if t.is_leaf:
+                with torch.no_grad():
+                    call(t)
+        call(trained.detach().clone())
+        with fwd.dual_level(), pytest.raises(RuntimeError, match="not differentiable"):
+            call(fwd.make_dual(x.clone(), x))
+    fa.check_status(0)
+
+
 def test_wait_that_runs_out_is_reported():
     # nothing is loaded: the waits of the kernel for many rows run out, the context stays usable
     import ctypes
