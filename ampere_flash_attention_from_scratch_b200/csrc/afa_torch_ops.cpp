@@ -376,7 +376,7 @@ AfaCache4 cache_args(const at::Tensor& cache, const at::Tensor& page_table, cons
 
 at::Tensor cache4_empty(int64_t n_pages, int64_t n_kv_heads, int64_t page_size, int64_t head_dim,
                         const std::optional<at::Device>& device) {
-  const int32_t row = afa_cache4_row_bytes(static_cast<int32_t>(head_dim));
+  const int32_t row = head_dim > 0 && head_dim <= INT32_MAX ? afa_cache4_row_bytes(static_cast<int32_t>(head_dim)) : -1;
   TORCH_CHECK(row > 0, "no sm_100a kernel for head_dim ", head_dim, " (64 and 128 are compiled)");
   TORCH_CHECK(n_pages > 0 && n_kv_heads > 0, "n_pages and n_kv_heads must be positive");
   TORCH_CHECK(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0,

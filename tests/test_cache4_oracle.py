@@ -108,6 +108,12 @@ def test_cache4_empty_refusals(args, match):
         fa.cache4_empty(*args, torch.device("cpu"))
 
 
+@pytest.mark.parametrize("wrap", [2 ** 32, -2 ** 32, 2 ** 40])
+def test_cache4_empty_head_dim_beyond_32_bits(wrap):
+    with pytest.raises(RuntimeError, match="head_dim"):
+        fa.cache4_empty(1, 1, 16, 64 + wrap, torch.device("cpu"))
+
+
 def test_package_exports_the_operators():
     import ampere_flash_attention_from_scratch_b200 as pkg
 
