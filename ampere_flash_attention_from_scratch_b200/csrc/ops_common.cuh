@@ -109,16 +109,18 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 // 32 bytes at a time: the row strides and addresses are multiples of 16, so where
-// the address is not one of 32 they go as two halves.  kReadOnly: nothing writes
-// that memory while the kernel runs.
-template <bool kReadOnly>
+// the address is not one of 32 they go as two halves.  kOnce: read by no other
+// thread, so not kept in L1.  (Not by ld.global.nc either way: the kernel is on the
+// GPU while the one before it still writes what it will read.)
+template <bool kOnce>
 __device__ __forceinline__ void load32(uint32_t (&v)[2][4], const char* p) {
   if ((reinterpret_cast<uintptr_t>(p) & 31u) == 0u) {
-    if constexpr (kReadOnly)
-      asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+    if constexpr (kOnce)
+      asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                    : "=r"(v[0][0]), "=r"(v[0][1]), "=r"(v[0][2]), "=r"(v[0][3]), "=r"(v[1][0]), "=r"(v[1][1]),
                      "=r"(v[1][2]), "=r"(v[1][3])
-                   : "l"(p));
+                   : "l"(p)
+                   : "memory");
     else
       asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                    : "=r"(v[0][0]), "=r"(v[0][1]), "=r"(v[0][2]), "=r"(v[0][3]), "=r"(v[1][0]), "=r"(v[1][1]),

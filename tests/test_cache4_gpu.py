@@ -898,6 +898,31 @@ def test_calls_in_a_row_see_each_other(capacity, n, HK):
     fa.check_status(0)
 
 
+@pytest.mark.parametrize("n", [1, 300])
+def test_rows_written_right_after_they_were_made(n):
+    # one buffer of keys, turned anew by the kernel before each write: no write sees the buffer's last contents
+    g = torch.Generator().manual_seed(n)
+    src = [torch.randn(4, n, 8, 128, generator=g).half().cuda() for _ in range(4)]
+    pos, inv = torch.arange(4 * n).view(1, 4, n).cuda(), torch.ones(64, device="cuda")
+    table, n_pages = pages([n] * 4, 64)
+    cache, table, lens = noise_cache(n_pages, 8, 64, 128).cuda(), table.cuda(), ints([n] * 4).cuda()
+    k = torch.empty_like(src[0])
+    want = []
+    for x in src:
+        fa.rotary(x, None, pos, inv, q_out=k)
+        torch.cuda.synchronize()
+        fa.cache4_write(k, k, cache, table, lens)
+        want.append(fa.cache4_read(cache, table, lens, n, torch.float16)[0])
+        torch.cuda.synchronize()
+    got = []
+    for i in range(100):
+        fa.rotary(src[i % 4], None, pos, inv, q_out=k)
+        fa.cache4_write(k, k, cache, table, lens)
+        got.append(fa.cache4_read(cache, table, lens, n, torch.float16)[0])
+    assert all(torch.equal(t, want[i % 4]) for i, t in enumerate(got))
+    fa.check_status(0)
+
+
 # --- together --------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_prompt_then_tokens(dtype):
