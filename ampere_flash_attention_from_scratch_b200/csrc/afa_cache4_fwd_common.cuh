@@ -73,7 +73,7 @@ __device__ __forceinline__ const char* far(const char* p, uint32_t n, uint32_t s
 // The division of the work, formed alike by every warp of both kernels
 // ---------------------------------------------------------------------------
 
-// Tokens of sequence b, 0 (reported) where the lengths are not possible.
+// Tokens of sequence b; 0 where no row needs them, or (reported) where the lengths are not possible.
 __device__ __forceinline__ int tokens_of(const FwdParams4& p, int b) {
   const int kv = p.c.kv_lens[b];
   const int fresh = p.c.new_lens != nullptr ? p.c.new_lens[b] : p.seq_len;
@@ -81,7 +81,7 @@ __device__ __forceinline__ int tokens_of(const FwdParams4& p, int b) {
     report(p.c.status, AFA_DEV_BAD_LENGTH);
     return 0;
   }
-  return kv;
+  return fresh == 0 ? 0 : kv;
 }
 // Units of an item: item_units that stand for what starting and ending an item
 // costs, then those of its tokens (one at least).

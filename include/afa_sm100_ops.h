@@ -91,7 +91,8 @@ typedef struct AfaCache4 {
   const int32_t* kv_lens;    /* [batch] tokens of each sequence, the new ones included */
   const int32_t* new_lens;   /* [batch] how many of the call's rows are new tokens of the
                                 sequence (the others are padding), or NULL: all of them.
-                                Row i < new_lens[b] is position kv_lens[b] - new_lens[b] + i */
+                                Row i < new_lens[b] is position kv_lens[b] - new_lens[b] + i.
+                                With none the sequence's pages are not looked at */
   int32_t* status;           /* optional, as AfaFwdArgs.status */
   int32_t n_pages;
   int32_t page_size; /* 16, 32, 64, 128 or 256 */

@@ -523,6 +523,25 @@ def test_bad_tables_and_lengths_are_reported(entry, fault):
         assert used == [False, True, False, False]
 
 
+@pytest.mark.parametrize("n", [3, 40])
+def test_idle_sequences_need_no_pages(n):
+    # a place of the batch without new rows keeps an old length, and its pages are gone
+    cache, table = filled([200, 90], 2, 128, 16, torch.float16, seed=n)
+    q = torch.randn(2, n, 4, 128, generator=torch.Generator().manual_seed(n)).half()
+    idle, new = table.clone(), [n, 0]
+    idle[1] = -1
+    for causal in (False, True):
+        o, lse = fa.forward_cache4(q.cuda(), cache.cuda(), idle.cuda(), ints([200, 90]).cuda(), None, causal, None, True, ints(new).cuda())
+        fa.check_status(0)
+        assert not o[1].any() and torch.all(lse[1] == -math.inf)
+        check_attention(q, cache, table, [200, 90], causal, new, got=(o, lse))
+    x = q[:, :, :2].cuda()
+    fa.cache4_write(x, x, cache.cuda(), idle.cuda(), ints([200, 90]).cuda(), ints(new).cuda())
+    k, v = fa.cache4_read(cache.cuda(), idle.cuda(), ints([200, 90]).cuda(), n, torch.float16, ints(new).cuda())
+    fa.check_status(0)
+    assert not k[1].any() and not v[1].any()
+
+
 def test_new_rows_beyond_the_sequence_are_refused_by_the_movers():
     # a sequence shorter than the rows to write has no place for them; attention allows it (rows that see nothing)
     cache = torch.zeros(2, 1, 2, 16, 36, dtype=torch.uint8, device="cuda")
