@@ -349,6 +349,25 @@ def test_nan_in_masked_places_stays_there(n):
         assert torch.isnan(o[:, -2:]).all()
 
 
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("n", [2, 45])
+def test_a_group_that_is_not_finite_leaves_the_other(n, value):
+    # one visible token's step of the values' first 64 channels: those are lost, the others and lse are not
+    lens = [300]
+    cache, table = filled(lens, 1, 128, 16, torch.bfloat16, seed=n)
+    q = torch.randn(1, n, 2, 128, generator=torch.Generator().manual_seed(1)).bfloat16()
+    want, want_lse, weight, reach = oc.attention64(q, cache, table, lens)
+    bad = cache.clone()
+    bad[table[0, 100 // 16], 0, 1, 100 % 16, 64:66] = torch.tensor([value], dtype=torch.bfloat16).view(torch.uint8)
+    o, lse = fa.forward_cache4(q.cuda(), bad.cuda(), table.cuda(), ints(lens).cuda(), return_lse=True)
+    fa.check_status(0)
+    o, lse = o.cpu().double(), lse.cpu().double()
+    assert not torch.isfinite(o[..., :64]).any()
+    tol = want.abs() * 2.0 ** -8 + (2.0 ** -11 + 2.0 ** -18 * reach[..., None] + 2.0 ** -15) * weight
+    assert torch.all(((o - want).abs() <= tol)[..., 64:])
+    assert torch.all((lse - want_lse).abs() <= 2.0 ** -19 * reach.transpose(1, 2) + 2.0 ** -15 + 2.0 ** -22 * want_lse.abs())
+
+
 def test_negative_steps_are_taken_as_written():
     # the format allows any s; rows from elsewhere may hold negative ones
     cache, table = filled([40], 1, 64, 16, torch.float16, seed=6)
