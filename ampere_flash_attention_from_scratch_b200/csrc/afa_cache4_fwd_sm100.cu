@@ -20,19 +20,23 @@
 //   * p, its sum, the running maximum and both accumulators are fp32.
 //
 // Bound.  HBM would be: 1.125 bytes a channel and token for keys and values.  The
-// kernel gets to three quarters of it for long contexts, and to the issue rate
-// first: 16 tokens of 128 channels take a warp 279 instructions -- 75 masks, 25
-// shifts and permutes, 16 matrix instructions, 45 fp32 operations -- and on this
-// sub-partition a mask takes 2 cycles, a matrix instruction 8 in which no fp32
-// operation issues: 510 cycles together, with as many warps as fit, from L2 or
-// from HBM alike.  Hence tokens on the M side of mma.m16n8k16 (16 tokens x 8 query
+// kernel gets to 70 to 80 % of it for long contexts: 16 tokens of 128 channels take a
+// warp 273 instructions -- some 75 masks, 25 shifts and permutes, 16 matrix
+// instructions, 45 fp32 operations -- in 510 cycles of a sub-partition with as many
+// warps as fit, from L2 or from HBM alike.  No one pipe is full (ALU 52 %, HMMA 26 %,
+// issue slots 55 %): a mask takes 2 cycles and a matrix instruction 8, under which fp32
+// operations find half their room (microbench/mma_sync_beside_alu.cu), and three warps
+// do not fill the gaps.  Hence tokens on the M side of mma.m16n8k16 (16 tokens x 8 query
 // rows): one row and eight cost the same, and no lane idles on a row block padded
 // to 128, for which the codes would also have to be spread in shared memory.
-// Measured: [8 x 131072 tokens, 32/8 heads, 128] bf16 240 us = 5.0 TB/s (77 % of the
-// measured copy bandwidth; 203 us with the arithmetic left out); [32 x 256..8192,
-// 32/8, 128] bf16 41 us = 3.8 TB/s; [16 x 250..4001, 32/32, 64] fp16 31 us = 2.6
-// TB/s (one of eight columns used, half the channels for the same softmax).
-// 500 tokens: 8 us on the device, the work's division, two dependent loads and
+// Measured: [8 x 131072 tokens, 32/8 heads, 128] bf16 261 us among other work = 4.6 TB/s
+// (71 % of the measured copy bandwidth), 231 us in calls in a row (a version that took
+// 240 took 203 with the arithmetic left out); among other work [32 x 256..8192, 32/8,
+// 128] bf16 41 us = 3.8 TB/s, [16 x 250..4001, 32/32, 64] fp16 31 us = 2.6 TB/s (one
+// of eight columns used, half the channels for the same softmax), [16 x 1024..16384, 5
+// new tokens, 64/8, 128] fp16 154 us (three blocks of 16 rows; at 16 rows and head_dim
+// 128 a thread has all 255 registers, and in bf16 20 bytes of them are spilled).
+// 500 tokens: 8.3 us on the device, the work's division, two dependent loads and
 // four steps of a warp.  4 CTAs an SM instead of 3 and 4 steps in the ring instead of 3: equal
 // to 3 % slower.
 //
@@ -787,9 +791,16 @@ int plan4(const AfaCache4* c, int32_t seq_len, int32_t n_heads, const Kernel4** 
   if (seq_len <= 0 || n_heads <= 0 || n_heads % c->n_kv_heads != 0) return AFA_ERR_INVALID_ARGUMENT;
   const int64_t rows = int64_t{seq_len} * (n_heads / c->n_kv_heads);
   if (rows > INT32_MAX - 64) return AFA_ERR_TOO_LARGE;
-  // mma.sync takes 51 us for every 16 rows of [16 sequences of 512..16384 tokens, 8 key/value heads, 128] fp16,
-  // tcgen05 181 us for 64 rows and 240 us for 128 (d 64: 30, 128 and 175); below about 1000 tokens a sequence the
-  // second starts and ends more slowly (34 us against 21 at one sequence of 2000 tokens, 64 rows).
+  // mma.sync repeats its unpacking for every 16 rows; tcgen05 does it once for 128, but starts and ends more slowly.
+  // Both, us, 8 key/value heads, fp16:
+  //   sequences x tokens      16 x 16384  16 x 4000  16 x 1000  4 x 4000  4 x 1000  1 x 2000
+  //   d 128,  48 rows          272 / 286   84 / 100    36 / 53   30 / 45   17 / 33   17 / 27
+  //           64               359 / 288  107 / 102    43 / 55   36 / 46   20 / 34   16 / 29
+  //          128               703 / 396  201 / 134    76 / 68   60 / 58   26 / 41   18 / 33
+  //   d 64,   64               201 / 203    62 / 72    27 / 39   24 / 34   14 / 25   15 / 20
+  //          128               388 / 270   112 / 93    44 / 49   37 / 43   19 / 31   15 / 24
+  // One border for all is a compromise: it loses up to a fifth at 49 to 64 rows of many long sequences, and up to half
+  // at 65 to 128 rows of short ones.  The lengths are on the device; the table's capacity bounds them and would tell.
   const int di = c->head_dim == 128, ti = c->dtype == AFA_DTYPE_BF16, ni = rows > 64 ? 2 : rows > 8;
   const Kernel4& k = kKernels4[di][ti][ni];
   const int64_t tiles = (rows + k.rows - 1) / k.rows;
@@ -817,6 +828,7 @@ int plan4(const AfaCache4* c, int32_t seq_len, int32_t n_heads, const Kernel4** 
   // Short sequences, few of them: one CTA an item.  The host then launches one kernel instead of two (7.5 us a call
   // instead of 9.8), and on the device 32/8 heads of 128 in bf16 take, split -> whole, us in a row: 32 sequences of
   // 500 tokens 16.4 -> 12.3, 1 of 500 10.2 -> 10.2, 1 of 1000 10.3 -> 12.7.  The tcgen05 kernel keeps the split.
+  // It is the table's width that counts: the same 32 sequences by tables of 131072 tokens take 15.2.
   *whole = ni < 2 && int64_t{c->max_pages} * c->page_size <= kWholeTokens && items * c->batch <= *grid;
   // no more CTAs than units at the sequences' largest possible lengths
   const int64_t most = *whole ? items * c->batch : units * items * c->batch;

@@ -13,8 +13,8 @@
 // minimum and maximum travel together as one packed pair through two shuffles.  A CTA
 // takes a tile of tokens of one sequence times (head, keys or values), tokens
 // fastest, so that the rows it writes are neighbours in a page.
-// Measured: reading back 131072 tokens [8, 128] bf16 109 us = 6.3 TB/s (96 % of
-// the measured copy bandwidth).  Eight prompts of 4096 down to 2304 tokens
+// Measured: reading back 131072 tokens [8, 128] bf16 117 us among other work = 5.9
+// TB/s (90 % of the measured copy bandwidth), 109 us in calls in a row.  Eight prompts of 4096 down to 2304 tokens
 // [8, 128] fp16, written and read back: 66 us = 4.5 TB/s (69 %); the reader is
 // at the bandwidth there too, the writer at its arithmetic (about 17
 // instructions a value, 69 % of the issue slots), so one row a lane (83 us) and

@@ -12,9 +12,10 @@
 // left is the softmax: about 15 instructions a row and token, and the broadcast of
 // a token's eight steps and minima to a warp, 8 shared-memory wavefronts (55 % of
 // the pipe; packed fp32 instructions therefore change nothing).
-// Measured: [1, 512 new of 131072 tokens, 32/8 heads, 128] bf16 2.86 ms = 384 TFLOP/s;
-// [16 x 512..16384, 8 key/value heads x 128 rows, 128] fp16 240 us, where the other
-// kernel takes 410.
+// Measured, in calls in a row: [1, 512 new of 131072 tokens, 32/8 heads, 128] bf16 2.85
+// ms = 386 TFLOP/s; [16 x 1024..16384, 8 key/value heads x 128 rows, 128] fp16 232 us,
+// where the other kernel takes 391.  Two CTAs an SM leave a thread 128 registers: 88
+// bytes are spilled at head_dim 128, 8 at 64.
 //
 //   warps 0-3   softmax: thread = row = TMEM lane; warp 0 also issues the MMAs
 //   warps 4-7   loads (cp.async ring), codes -> fp16 tiles, steps and minima

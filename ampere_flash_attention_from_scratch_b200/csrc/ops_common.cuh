@@ -49,9 +49,11 @@ inline int ops_launched() {
 
 // A launch whose CTAs may take their places while the stream's kernel before
 // it ends; the kernel calls after_previous() before it touches global memory.
-// Calls in a row, plain -> so: rotary of 64 tokens 4.1 -> 2.7 us, a token
-// written to 128 sequences and read back 8.2 -> 5.2, attention over 500 tokens
-// 10.3 -> 8.0; the large cases lose 2 to 3 us; the host's side is no longer.
+// Calls in a row, plain -> so: rotary of 64 tokens 4.2 -> 2.8 us, a token
+// written to 128 sequences and read back 8.3 -> 5.2, attention over 500 tokens
+// 10.3 -> 8.3, over 32 x 256..8192 45.9 -> 41.9, over 8 x 131072 237 -> 231; 8
+// prompts written and read back 70.4 -> 66.5, 131072 tokens read back 110.7 ->
+// 109.3.  Among other work no case is slower either (8 x 131072 264 -> 262).
 template <class... P, class... A>
 inline cudaError_t ops_launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s,
                               const A&... args) {

@@ -9,7 +9,8 @@
  * As in afa_sm100.h: plain C types, device pointers, a cudaStream_t passed as
  * void*; no call allocates, frees or synchronises; every entry point returns
  * an AFA_* code, checks its arguments before any CUDA call and never throws.
- * Every wait inside a kernel is bounded, as there.
+ * Every wait for a barrier inside a kernel is bounded, as there; the allocation
+ * of tensor memory waits as long as kernels of other streams hold it.
  *
  * The cache.  One uint8 array [n_pages][n_kv_heads][2][page_size][row] (index
  * 2: keys, values), row = head_dim / 2 + head_dim / 16 bytes: 36 at head_dim
@@ -129,10 +130,11 @@ int afa_cache4_read_sm100(const AfaCache4* cache, void* k, void* v, const int64_
  * kv_lens[b] - new_lens[b] + i.  A row that sees no token and a padding row
  * get O = 0 and lse = -inf.  A NaN among a row's visible keys makes the row NaN,
  * one among its visible values the 64 channels of its group; a masked token does
- * nothing, whatever it holds.  Queries are exact up to 2^110 in magnitude.  A
- * token's weight times each of its two values' steps is held in fp16, measured by
- * the largest such product of the row: 2^-11 relative down to 2^-21 of that, and
- * below to 2^-32 of it.  Steps may go up to 2^100; where all of a row's lie below
+ * nothing, whatever it holds.  Queries are exact where a row's largest element is
+ * from 2^-77 to 2^110, elements down to 2^-23 of it, and to 2^-34 of it below.  A
+ * token's weight times each of its values' steps is held in fp16, measured by the
+ * largest such product of the row: to 2^-11 relative down to 2^-21 of that, and to
+ * 2^-32 of it below.  Steps may go up to 2^100; where all of a row's lie below
  * 2^-81 they lose bits.  Calls of more than 64 query rows a key/value head (seq_len * n_heads /
  * n_kv_heads) run on tcgen05, others on mma.sync. */
 typedef struct AfaCache4FwdArgs {
