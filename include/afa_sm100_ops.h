@@ -135,8 +135,8 @@ int afa_cache4_read_sm100(const AfaCache4* cache, void* k, void* v, const int64_
  * token's weight times each of its values' steps is held in fp16, measured by the
  * largest such product of the row: to 2^-11 relative down to 2^-21 of that, and to
  * 2^-32 of it below.  Steps may go up to 2^100; where all of a row's lie below
- * 2^-81 they lose bits.  Calls of more than 64 query rows a key/value head (seq_len * n_heads /
- * n_kv_heads) run on tcgen05, others on mma.sync. */
+ * 2^-81 they lose bits.  Calls of more than 64 query rows a key/value head
+ * (seq_len * n_heads / n_kv_heads) run on tcgen05, others on mma.sync. */
 typedef struct AfaCache4FwdArgs {
   const void* q;
   void* o;
